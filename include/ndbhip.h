@@ -95,6 +95,11 @@ int			ndbhip_set_stream(void *hip_stream);
  * HIP call (bench.py sets it for itself; under rocprofv3 export it in the shell: tools/round_profiles.sh). */
 int			ndbhip_set_thread_stream(void *hip_stream);
 int			ndbhip_get_stream(void **out_hip_stream);	/* the stream every asynchronous entry point is ordered on */
+/* The calling thread's stream for a stretch of calls: sets it as ndbhip_set_thread_stream does and hands back what it was
+ * (NULL: the process-wide one), to be set again afterwards.  NDBHIP_STREAM_LEGACY stands for the legacy default stream,
+ * whose own handle is 0. */
+#define NDBHIP_STREAM_LEGACY ((void *) 1)
+int			ndbhip_swap_thread_stream(void *hip_stream, void **out_previous);
 int			ndbhip_synchronize(void);
 
 /* Per-process counters (replaces GPUStats, include/neurondb_gpu.h:34-42). */
@@ -730,6 +735,81 @@ int			ndbhip_pair_distance(const float *A, const float *B, float *out, int n, in
 int			ndbhip_kmeans_assign(const float *X, const float *C, int *idx, int n, int dim, int k);
 int			ndbhip_kmeans_update(const float *X, const int *idx, float *C, int n, int dim, int k);
 int			ndbhip_quant_fp16(const float *in, uint16_t *out, int64_t n);
+
+/* ------------------------------------------------------------------ */
+/* 8-bit tables and scores (new surface; the reference has the int8 codec  */
+/* only: launch_quant_int8 of its GPU vtable takes ONE scale for a whole   */
+/* table).  RN = round to nearest even, fp32 unless said otherwise.        */
+/*                                                                         */
+/*   bytes      a row x becomes signed bytes and one fp32 scale: top = max |x|; top < 2^-100: scale 0, bytes 0; a NaN or an
+ *              infinity in the row: scale NaN, bytes 0; else scale = RN(top / 127) and byte = the integer nearest to
+ *              x * RN(127 / top), that product taken exactly, halves to even (-127 .. 127)
+ *   score      of row i for query q: RN(RN(RN(dot) * scale_i) * scale_q), dot the exact int32 sum of the bytes' products;
+ *              then RN(score + bias_i) where a bias is given.  Queries are quantised inside the call like rows, unless they
+ *              come as NDBHIP_I8 with their scales.  Higher is better: this is the inner product (for rows and queries of
+ *              norm 1 the cosine; a bias of -|x_i|^2 / 2 orders rows by L2 distance).
+ *   bias       [n] fp32
+ *   mask       bit i % 32 of word i / 32: 1 = row i may be returned.  mask_stride: words from one query's mask to the next
+ *              (>= (n + 31) / 32), 0 = one mask for all queries
+ *
+ * Device pointers unless said otherwise; asynchronous on the library's stream (ndbhip_set_stream,
+ * ndbhip_set_thread_stream), capturable into a graph.  Strides are in elements.  Nothing is kept between calls: a table
+ * is only read, so any number of threads and streams may use one table at the same time, each call with a workspace of its own
+ * (ndbhip_i8_workspace; 256-byte aligned; its contents mean nothing before or after, and it must live until the call's kernels
+ * have run — for a captured graph, as long as the graph is replayed).  ndbhip_i8_load* and _destroy wait for nothing but
+ * their own work: call them while no other call on the table is in flight and no graph that reads it will be replayed.
+ * Any dimension 1 .. 32767, any number of rows below 2^31 - 256, any strides and alignments of an element's own size
+ * (rows on 16-byte boundaries are read fastest). */
+/* ------------------------------------------------------------------ */
+typedef struct ndbhip_i8 ndbhip_i8;		/* device-resident table of 8-bit rows */
+
+#define NDBHIP_F32   0
+#define NDBHIP_F16   1
+#define NDBHIP_BF16  2
+#define NDBHIP_I8    3
+
+/* rows -> bytes and scales; bytes and scales -> values (RN(byte * scale), rounded once more to a 16-bit type) */
+int			ndbhip_i8_quantize_device(const void *d_x, int dtype, int64_t nrows, int dim, int64_t x_stride,
+									  int8_t *d_codes, int64_t codes_stride, float *d_scales);
+int			ndbhip_i8_dequantize_device(const int8_t *d_codes, int64_t codes_stride, const float *d_scales, int64_t nrows, int dim,
+										void *d_out, int dtype, int64_t out_stride);
+
+int			ndbhip_i8_create(int dim, ndbhip_i8 **out);
+int			ndbhip_i8_destroy(ndbhip_i8 *t);
+/* The table's rows, in place of what it held (which is gone also when the load fails): from host float4 rows [nrows][dim],
+ * or from device rows of any of the types; d_scales goes with NDBHIP_I8 rows and is NULL otherwise.  Both return when the
+ * rows are in the table. */
+int			ndbhip_i8_load(ndbhip_i8 *t, const float *rows, int64_t nrows);
+int			ndbhip_i8_load_device(ndbhip_i8 *t, const void *d_rows, int dtype, int64_t nrows, int64_t row_stride, const float *d_scales);
+int			ndbhip_i8_export_device(const ndbhip_i8 *t, int8_t *d_codes, int64_t codes_stride, float *d_scales);
+int64_t		ndbhip_i8_nrows(const ndbhip_i8 *t);
+int			ndbhip_i8_dim(const ndbhip_i8 *t);
+/* bytes of workspace for a batch of nq queries: k = 0 for ndbhip_i8_product_device, the search's k for a search */
+int			ndbhip_i8_workspace(const ndbhip_i8 *t, int nq, int k, size_t *bytes);
+
+/* every score: d_out[q * out_stride + i], fp32 or rounded once more to 16 bits */
+int			ndbhip_i8_product_device(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_q_scales, int nq, int64_t q_stride,
+									 const float *d_bias, void *d_out, int out_type, int64_t out_stride, void *d_ws, size_t ws_bytes);
+/* The k (1 .. NDBHIP_MAX_K) best rows of each query: ids [nq][k] and scores [nq][k], higher scores first and equal scores (-0
+ * and 0 among them) in the order of their ids.  A row takes part where its mask bit is 1 and its score is neither NaN nor
+ * -infinity; places that no row fills hold id -1 and score -infinity. */
+int			ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_q_scales, int nq, int64_t q_stride,
+									const float *d_bias, const uint32_t *d_mask, int64_t mask_stride, int k, int64_t *d_ids, float *d_scores,
+									void *d_ws, size_t ws_bytes);
+/* the same for host queries [nq][dim] and host bias, mask and results */
+int			ndbhip_i8_search(const ndbhip_i8 *t, const float *queries, int nq, const float *bias, const uint32_t *mask, int64_t mask_stride,
+							 int k, int64_t *ids, float *scores);
+
+/* Penalties, biases and masks over a matrix of scores [nq][n] (fp32, fp16 or bf16; arithmetic in fp32, rounded once), to
+ * another matrix of the type or in place (d_out == d_scores with the same stride; no other overlap):
+ *   seen       query q has been given ids d_seen_ids[d_seen_off[q] .. d_seen_off[q + 1]) before, in any order, an id once for
+ *              every time; ids outside 0 .. n - 1 count for nothing.  d_penalties[q] = {repeat, presence, frequency}, repeat > 0.  For an id
+ *              given c > 0 times: s = s > 0 ? s / repeat : s * repeat, then s = s - (presence + c * frequency).  d_seen_off NULL: none
+ *   bias       s = s + bias; bias_stride from one query's to the next, 0 = one for all; NULL: none
+ *   mask       bit 0: s = -infinity, whatever it was; as above; NULL: none */
+int			ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, int64_t stride, const int64_t *d_seen_off,
+										const int32_t *d_seen_ids, const float *d_penalties, const float *d_bias, int64_t bias_stride,
+										const uint32_t *d_mask, int64_t mask_stride, void *d_out, int64_t out_stride);
 
 #ifdef __cplusplus
 }

@@ -9,5 +9,7 @@ and raises if the library is missing.
 from ._lib import NdbHipError, lib, lib_path, last_error  # noqa: F401
 from .ivf import IvfIndex, IvfScan  # noqa: F401
 from .hnsw import HnswIndex, HnswScan  # noqa: F401
+from .int8 import Int8Table, adjust_scores, dequantize_rows, quantize_rows  # noqa: F401
 
-__all__ = ["NdbHipError", "lib", "lib_path", "last_error", "IvfIndex", "IvfScan", "HnswIndex", "HnswScan"]
+__all__ = ["NdbHipError", "lib", "lib_path", "last_error", "IvfIndex", "IvfScan", "HnswIndex", "HnswScan",
+           "Int8Table", "quantize_rows", "dequantize_rows", "adjust_scores"]

@@ -155,6 +155,21 @@ def lib():
         "ndbhip_set_scan_mode": (i, [i]),
         "ndbhip_set_option": (i, [C.c_char_p, i]),
         "ndbhip_set_thread_stream": (i, [vp]),
+        "ndbhip_swap_thread_stream": (i, [vp, C.POINTER(vp)]),
+        "ndbhip_i8_quantize_device": (i, [vp, i, i64, i, i64, vp, i64, vp]),
+        "ndbhip_i8_dequantize_device": (i, [vp, i64, vp, i64, i, vp, i, i64]),
+        "ndbhip_i8_create": (i, [i, C.POINTER(vp)]),
+        "ndbhip_i8_destroy": (i, [vp]),
+        "ndbhip_i8_load": (i, [vp, vp, i64]),
+        "ndbhip_i8_load_device": (i, [vp, vp, i, i64, i64, vp]),
+        "ndbhip_i8_export_device": (i, [vp, vp, i64, vp]),
+        "ndbhip_i8_nrows": (i64, [vp]),
+        "ndbhip_i8_dim": (i, [vp]),
+        "ndbhip_i8_workspace": (i, [vp, i, i, C.POINTER(C.c_size_t)]),
+        "ndbhip_i8_product_device": (i, [vp, vp, i, vp, i, i64, vp, vp, i, i64, vp, C.c_size_t]),
+        "ndbhip_i8_search_device": (i, [vp, vp, i, vp, i, i64, vp, vp, i64, i, vp, vp, vp, C.c_size_t]),
+        "ndbhip_i8_search": (i, [vp, vp, i, vp, vp, i64, i, vp, vp]),
+        "ndbhip_scores_adjust_device": (i, [vp, i, i, i64, i64, vp, vp, vp, vp, i64, vp, i64, vp, i64]),
         "ndbhip_mfma_probe": (i, [vp, vp, vp, vp, i, i]),
         "ndbhip_mfma_probe_f32": (i, [vp, vp, vp, vp, i]),
         "ndbhip_debug_phases": (i, [vp]),

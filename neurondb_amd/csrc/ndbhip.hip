@@ -325,6 +325,17 @@ ndbhip_set_thread_stream(void *s)
 }
 
 extern "C" int
+ndbhip_swap_thread_stream(void *s, void **prev)
+{
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (!prev)
+		return fail(NDBHIP_ERR_INVALID, "out is NULL");
+	*prev = (void *) ndbhip_tl_stream;
+	ndbhip_tl_stream = (hipStream_t) s;
+	return NDBHIP_OK;
+}
+
+extern "C" int
 ndbhip_get_stream(void **out_hip_stream)
 {
 	if (need_init()) return NDBHIP_ERR_NODEVICE;

@@ -1,0 +1,1333 @@
+/*
+ * ndbhip_int8.hip — the 8-bit half of libndbhip.so: rows quantised to signed bytes with one scale each, the int8
+ * matrix product of queries with a table of such rows, penalties / biases / masks over a matrix of scores, and the k
+ * best rows of a table for every query.  Host entry points of include/ndbhip.h ("8-bit tables and scores").
+ * Written for wave64 / CDNA4 (gfx950) only.
+ *
+ * Layout.  A table (and a batch of queries while a call runs) is kept in blocks of 32 rows; inside a block the
+ * dimensions go in slices of 16: unit (row r, slice t) = 16 bytes at t * 512 + (r % 32) * 16.  Two neighbouring slices
+ * are 1 KiB, and lane l of a wave reading 16 bytes at 16 l holds exactly what v_mfma_i32_32x32x32_i8 takes from lane l
+ * as the A (or B) operand: row l % 32, bytes 16 (l / 32) .. + 15 of the 32.  So an operand is one contiguous KiB, from
+ * memory or from LDS, with no shuffle and no bank conflict, and a block is one contiguous stream.  Dimensions are padded
+ * with zeros to a multiple of 64, rows to a multiple of 256; a padding row's scale is NaN, which no search returns.
+ */
+#include "ndbhip_internal.h"
+#include <hip/hip_fp16.h>
+#include <hip/hip_bf16.h>
+#include <new>
+
+typedef int i8_v4i __attribute__((ext_vector_type(4)));
+typedef int i8_v16i __attribute__((ext_vector_type(16)));
+
+#define I8_ROW_PAD	256u		/* rows of a table are laid out in multiples of this (the widest tile) */
+#define I8_DIM_PAD	64u
+/* a row whose largest magnitude is below this is a row of zeros: 127 / top must stay finite */
+#define I8_TINY		0x1p-100f
+#define I8_NINF		(-__builtin_inff())
+
+__host__ __device__ __forceinline__ uint32_t
+i8_up(uint32_t v, uint32_t to)
+{
+	return (v + to - 1) / to * to;
+}
+
+/* ================================================================== */
+/* element types                                                       */
+/* ================================================================== */
+
+template <class T> struct I8Elem;
+template <> struct I8Elem<float>
+{
+	static __device__ __forceinline__ float load(float v) { return v; }
+	static __device__ __forceinline__ float store(float v) { return v; }
+};
+template <> struct I8Elem<__half>
+{
+	static __device__ __forceinline__ float load(__half v) { return __half2float(v); }
+	static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
+};
+template <> struct I8Elem<__hip_bfloat16>
+{
+	static __device__ __forceinline__ float load(__hip_bfloat16 v) { return __bfloat162float(v); }
+	static __device__ __forceinline__ __hip_bfloat16 store(float v) { return __float2bfloat16(v); }
+};
+
+template <class T, int N> struct alignas(sizeof(T) * N) I8Vec
+{
+	T			v[N];
+};
+
+/* ================================================================== */
+/* quantise / dequantise                                               */
+/* ================================================================== */
+
+/*
+ * byte = the integer nearest to x * inv, inv = RN(127 / top), halves to even.  One fused multiply-add onto 1.5 * 2^23
+ * rounds the EXACT product to an integer once — RN(x * inv) first and rounding that would move products just beside a
+ * half onto it — and leaves the integer in the low mantissa bits, whose low byte is the signed byte.
+ */
+__device__ __forceinline__ uint32_t
+i8_byte(float x, float inv)
+{
+	return __float_as_uint(__builtin_fmaf(x, inv, 12582912.0f)) & 255u;
+}
+
+/*
+ * L lanes (a power of two) hold a row, 64 / L rows a wave; a lane takes VEC neighbouring elements (16 bytes of input)
+ * at a time.  The row's largest magnitude is an integer maximum over the magnitude bits, in which NaN and infinity are
+ * largest and so cannot be lost.  Rows of up to CH * L * VEC elements stay in registers between the two passes; longer
+ * ones are read again (from L2).  BLOCKED: bytes go to the block layout (rows from nrows on: zeros, scale NaN), else
+ * to rows of `cstride` bytes.  Bound by HBM: e bytes read and one written per element.
+ */
+template <class T, bool BLOCKED, int CH>
+__global__ __launch_bounds__(256) void
+k_i8_quantize(const T *__restrict__ x, int64_t nrows, int64_t nrows_out, int dim, int64_t xstride, int lanes_log2, int xvec,
+			  unsigned char *__restrict__ codes, int64_t cstride, int cvec, uint32_t kp, float *__restrict__ scales)
+{
+	constexpr int VEC = 16 / sizeof(T);
+	const int	L = 1 << lanes_log2;
+	const int	lane = threadIdx.x & (L - 1);
+	const int64_t row = (int64_t) blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2);
+	const bool	real = row < nrows;
+	const T    *p = x + (real ? row : 0) * xstride;
+	const int	step = L * VEC;
+
+	auto		load = [&](int e, float (&f)[VEC]) {
+		if (real && xvec && e + VEC <= dim)
+		{
+			const I8Vec<T, VEC> v = *(const I8Vec<T, VEC> *) (p + e);
+
+#pragma unroll
+			for (int i = 0; i < VEC; i++)
+				f[i] = I8Elem<T>::load(v.v[i]);
+		}
+		else
+#pragma unroll
+			for (int i = 0; i < VEC; i++)
+				f[i] = real && e + i < dim ? I8Elem<T>::load(p[e + i]) : 0.0f;
+	};
+	float		reg[CH][VEC];
+	uint32_t	top = 0;
+
+	if (CH * step >= dim)
+	{
+#pragma unroll
+		for (int c = 0; c < CH; c++)
+			load(c * step + lane * VEC, reg[c]);
+#pragma unroll
+		for (int c = 0; c < CH; c++)
+#pragma unroll
+			for (int i = 0; i < VEC; i++)
+				top = max(top, __float_as_uint(reg[c][i]) & 0x7FFFFFFFu);
+	}
+	else
+		for (int e = lane * VEC; e < dim; e += step)
+		{
+			load(e, reg[0]);
+#pragma unroll
+			for (int i = 0; i < VEC; i++)
+				top = max(top, __float_as_uint(reg[0][i]) & 0x7FFFFFFFu);
+		}
+	for (int off = L >> 1; off > 0; off >>= 1)
+		top = max(top, (uint32_t) __shfl_xor((int) top, off, 64));
+
+	const float ftop = __uint_as_float(top);
+	const bool	finite = top < 0x7F800000u;
+	const bool	live = finite && ftop >= I8_TINY;
+	const float inv = live ? 127.0f / ftop : 0.0f;
+
+	if (lane == 0 && row < nrows_out)
+		scales[row] = !real || !finite ? __builtin_nanf("") : live ? ftop / 127.0f : 0.0f;
+	if (row >= nrows_out)
+		return;
+
+	unsigned char *out = BLOCKED ? codes + (size_t) (row >> 5) * 32u * kp + (row & 31) * 16u : codes + row * cstride;
+	auto		put = [&](int e, const float (&f)[VEC]) {
+		uint32_t	w[VEC / 4];
+
+#pragma unroll
+		for (int i = 0; i < VEC / 4; i++)
+			w[i] = live ? i8_byte(f[4 * i], inv) | i8_byte(f[4 * i + 1], inv) << 8 | i8_byte(f[4 * i + 2], inv) << 16 |
+				i8_byte(f[4 * i + 3], inv) << 24 : 0u;
+		if (BLOCKED)
+		{
+			unsigned char *o = out + (size_t) (e >> 4) * 512u + (e & 15);
+
+			if (VEC == 4)
+				*(uint32_t *) o = w[0];
+			else
+				*(uint2 *) o = make_uint2(w[0], w[VEC / 4 - 1]);
+		}
+		else if (cvec && e + VEC <= dim)
+		{
+			if (VEC == 4)
+				*(uint32_t *) (out + e) = w[0];
+			else
+				*(uint2 *) (out + e) = make_uint2(w[0], w[VEC / 4 - 1]);
+		}
+		else
+#pragma unroll
+			for (int i = 0; i < VEC; i++)
+				if (e + i < dim)
+					out[e + i] = (unsigned char) (w[i / 4] >> (8 * (i % 4)));
+	};
+	const int	end = BLOCKED ? (int) kp : dim;
+
+	if (CH * step >= dim)
+	{
+#pragma unroll
+		for (int c = 0; c < CH; c++)
+			if (c * step + lane * VEC < end)
+				put(c * step + lane * VEC, reg[c]);
+		if (BLOCKED)			/* padding dimensions beyond the registers' reach */
+			for (int e = CH * step + lane * VEC; e < end; e += step)
+			{
+				load(e, reg[0]);
+				put(e, reg[0]);
+			}
+	}
+	else
+		for (int e = lane * VEC; e < end; e += step)
+		{
+			load(e, reg[0]);
+			put(e, reg[0]);
+		}
+}
+
+/* byte * scale in fp32, rounded once more where the output has 16 bits; a thread takes four elements */
+template <class T>
+__global__ __launch_bounds__(256) void
+k_i8_dequantize(const int8_t *__restrict__ codes, int64_t cstride, int cvec, const float *__restrict__ scales, int64_t nrows, int dim,
+				int lanes_log2, T *__restrict__ out, int64_t ostride, int ovec)
+{
+	const int	L = 1 << lanes_log2;
+	const int	lane = threadIdx.x & (L - 1);
+	const int64_t row = (int64_t) blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2);
+
+	if (row >= nrows)
+		return;
+	const int8_t *c = codes + row * cstride;
+	T		   *o = out + row * ostride;
+	const float s = scales[row];
+
+	for (int e = lane * 4; e < dim; e += 4 * L)
+	{
+		const int	m = min(4, dim - e);
+		uint32_t	w = 0;
+		I8Vec<T, 4> v;
+
+		if (cvec && m == 4)
+			w = *(const uint32_t *) (c + e);
+		else
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				w |= i < m ? (uint32_t) (uint8_t) c[e + i] << (8 * i) : 0u;
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+			v.v[i] = I8Elem<T>::store((float) (int8_t) (w >> (8 * i)) * s);
+		if (ovec && m == 4)
+			*(I8Vec<T, 4> *) (o + e) = v;
+		else
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				if (i < m)
+					o[e + i] = v.v[i];
+	}
+}
+
+/* rows of bytes <-> the block layout, 16 bytes a thread (neighbouring threads: neighbouring slices of a row) */
+template <bool PACK>
+__global__ __launch_bounds__(256) void
+k_i8_blocks(const unsigned char *__restrict__ src, unsigned char *__restrict__ dst, int64_t stride, int vec, int64_t nrows, int64_t nrows_out,
+			int dim, uint32_t kp, const float *__restrict__ sin, float *__restrict__ sout)
+{
+	const uint32_t slices = kp / 16;
+	const uint64_t unit = (uint64_t) blockIdx.x * 256 + threadIdx.x;
+	const int64_t row = unit / slices;
+	const int	e = (int) (unit - (uint64_t) row * slices) * 16;
+
+	if (row >= nrows_out)
+		return;
+	const size_t blk = (size_t) (row >> 5) * 32u * kp + (row & 31) * 16u + (size_t) (e >> 4) * 512u;
+	union { uint4 q; unsigned char b[16]; } u;
+
+	if (PACK)
+	{
+		const unsigned char *s = src + row * stride + e;
+
+		u.q = make_uint4(0, 0, 0, 0);
+		if (row < nrows && vec && e + 16 <= dim)
+			u.q = *(const uint4 *) s;
+		else if (row < nrows)
+			for (int i = 0; i < 16; i++)
+				if (e + i < dim)
+					u.b[i] = s[i];
+		*(uint4 *) (dst + blk) = u.q;
+	}
+	else
+	{
+		unsigned char *d = dst + row * stride + e;
+
+		u.q = *(const uint4 *) (src + blk);
+		if (vec && e + 16 <= dim)
+			*(uint4 *) d = u.q;
+		else
+			for (int i = 0; i < 16; i++)
+				if (e + i < dim)
+					d[i] = u.b[i];
+	}
+	if (e == 0)
+		sout[row] = row < nrows ? sin[row] : __builtin_nanf("");
+}
+
+/* ================================================================== */
+/* the product                                                         */
+/* ================================================================== */
+
+/* what becomes of a 32 x 32 block of sums: written as scores, or reduced to each query's largest of the 32 rows */
+struct I8Out
+{
+	const float *rscale;		/* [rows padded] */
+	const float *qscale;		/* [queries padded to 32] */
+	const float *bias;			/* [n] or NULL */
+	const uint32_t *mask;		/* bit i of word i / 32, or NULL */
+	int64_t		mask_stride;	/* words from one query to the next; 0 = one mask for all */
+	void	   *out;			/* scores */
+	int64_t		ostride;
+	int			ovec;			/* four scores may be stored at once */
+	float	   *gmax;			/* [nq][ngp]: the largest score of each block of 32 rows that takes part, -inf if none */
+	uint32_t	ngp;
+	uint32_t	n;
+	uint32_t	nq;
+};
+
+/* RN(RN(RN(dot) * row scale) * query scale) (+ bias): the definition's own roundings, so that equal scores are equal */
+__device__ __forceinline__ float
+i8_score(int dot, float rs, float qs)
+{
+	return ((float) dot * rs) * qs;
+}
+
+/*
+ * The block of sums of row block rb and query block qb: lane l has query l % 32 and, in register 4 g + j, row
+ * 8 g + 4 (l / 32) + j.
+ */
+template <class T>
+__device__ __forceinline__ void
+i8_write_scores(const I8Out &o, uint32_t rb, uint32_t qb, const i8_v16i &acc)
+{
+	const int	lane = threadIdx.x & 63;
+	const uint32_t q = qb * 32 + (lane & 31);
+	const uint32_t r0 = rb * 32 + 4 * (lane >> 5);
+
+	if (q >= o.nq)
+		return;
+	const float qs = o.qscale[q];
+	T		   *out = (T *) o.out + (int64_t) q * o.ostride;
+
+#pragma unroll
+	for (int g4 = 0; g4 < 4; g4++)
+	{
+		const uint32_t r = r0 + 8 * g4;
+		const float4 rs = *(const float4 *) (o.rscale + r);
+		float		s[4] = {i8_score(acc[4 * g4], rs.x, qs), i8_score(acc[4 * g4 + 1], rs.y, qs),
+			i8_score(acc[4 * g4 + 2], rs.z, qs), i8_score(acc[4 * g4 + 3], rs.w, qs)};
+		I8Vec<T, 4> v;
+
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+		{
+			if (o.bias && r + j < o.n)
+				s[j] = s[j] + o.bias[r + j];
+			v.v[j] = I8Elem<T>::store(s[j]);
+		}
+		if (o.ovec && r + 4 <= o.n)
+			*(I8Vec<T, 4> *) (out + r) = v;
+		else
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				if (r + j < o.n)
+					out[r + j] = v.v[j];
+	}
+}
+
+/* the largest score that takes part among the 32 rows of block rb, for the lane's query (both halves of the wave hold it) */
+__device__ __forceinline__ float
+i8_block_max(const I8Out &o, uint32_t rb, uint32_t q, const i8_v16i &acc)
+{
+	const int	lane = threadIdx.x & 63;
+	const uint32_t r0 = rb * 32 + 4 * (lane >> 5);
+	const bool	in = q < o.nq && rb * 32 < o.n;
+	const float qs = in ? o.qscale[q] : 0.0f;
+	const uint32_t bits = in && o.mask ? o.mask[(int64_t) q * o.mask_stride + rb] : 0xFFFFFFFFu;
+	float		m = I8_NINF;
+
+#pragma unroll
+	for (int g4 = 0; g4 < 4; g4++)
+	{
+		const uint32_t r = r0 + 8 * g4;
+		const float4 rs = *(const float4 *) (o.rscale + r);
+		const float rv[4] = {rs.x, rs.y, rs.z, rs.w};
+
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+		{
+			float		s = i8_score(acc[4 * g4 + j], rv[j], qs);
+
+			if (o.bias && r + j < o.n)
+				s = s + o.bias[r + j];
+			/* (a comparison with NaN is false: NaN scores, padding rows among them, never take part) */
+			if ((bits >> ((r + j) & 31) & 1u) && s > m)
+				m = s;
+		}
+	}
+	return fmaxf(m, __shfl_xor(m, 32, 64));
+}
+
+/* The simple form: a wave multiplies one block of 32 rows with TB blocks of 32 queries straight from memory. */
+template <int TB, int MODE, class T>
+__global__ __launch_bounds__(256) void
+k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrb, uint32_t nqb, I8Out o)
+{
+	const int	lane = threadIdx.x & 63;
+	const uint32_t rb = blockIdx.x * 4 + (threadIdx.x >> 6);
+	const uint32_t qb0 = blockIdx.y * TB;
+
+	if (rb >= nrb)
+		return;
+	const unsigned char *a = rows + (size_t) rb * 32u * kp + lane * 16;
+	const unsigned char *b = queries + (size_t) qb0 * 32u * kp + lane * 16;
+	i8_v16i		acc[TB];
+
+#pragma unroll
+	for (int t = 0; t < TB; t++)
+#pragma unroll
+		for (int i = 0; i < 16; i++)
+			acc[t][i] = 0;
+	for (uint32_t k = 0; k < kp; k += 32)
+	{
+		const i8_v4i av = *(const i8_v4i *) (a + (size_t) k * 32);
+
+#pragma unroll
+		for (int t = 0; t < TB; t++)
+			if (qb0 + t < nqb)
+				acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, *(const i8_v4i *) (b + (size_t) t * 32 * kp + (size_t) k * 32),
+															   acc[t], 0, 0, 0);
+	}
+#pragma unroll
+	for (int t = 0; t < TB; t++)
+		if (qb0 + t < nqb)
+		{
+			if (MODE == 0)
+				i8_write_scores<T>(o, rb, qb0 + t, acc[t]);
+			else
+			{
+				const uint32_t q = (qb0 + t) * 32 + (lane & 31);
+				const float m = i8_block_max(o, rb, q, acc[t]);
+
+				if (lane < 32 && q < o.nq)
+					o.gmax[(size_t) q * o.ngp + rb] = m;
+			}
+		}
+}
+
+/* ================================================================== */
+/* the k best                                                          */
+/* ================================================================== */
+
+/*
+ * Any k best rows lie in the k row blocks with the largest maxima (equal maxima: the lower block first): a row of
+ * another block has k rows ahead of it, one in each of those blocks.  So the product leaves one number per (query, 32
+ * rows), k blocks are picked, and only their rows are scored again — one by one, with the same roundings.
+ *
+ * k_i8_pick: a block of threads per query; picked[q][0 .. npicked[q]) in ascending order.
+ */
+__global__ __launch_bounds__(256) void
+k_i8_pick(const float *__restrict__ gmax, uint32_t ngp, uint32_t ng, uint32_t k, uint32_t *__restrict__ picked, uint32_t *__restrict__ npicked)
+{
+	__shared__ uint32_t hist[256], sh[16];
+	__shared__ uint64_t comp[NDBHIP_MAX_K];
+	__shared__ uint32_t pay[NDBHIP_MAX_K];
+	const uint32_t q = blockIdx.x;
+	const float *gm = gmax + (size_t) q * ngp;
+	auto		f = [&](uint32_t i, uint32_t &bits) -> bool {
+		const float m = gm[i];
+
+		bits = __float_as_uint(-m);
+		return m > I8_NINF;
+	};
+	uint32_t	T, less, kk, eq;
+
+	block_radix_select(f, ng, k, hist, sh, T, less, kk, eq);
+	if (threadIdx.x == 0)
+		npicked[q] = kk;
+	if (kk == 0)
+		return;
+	block_ordered_gather(f, ng, T, kk - less, sh, [&](int cls, uint32_t rank, uint32_t i, uint32_t) {
+		comp[cls == 0 ? rank : less + rank] = i;
+	});
+	__syncthreads();
+	uint32_t	npad = 1;
+
+	while (npad < kk)
+		npad <<= 1;
+	for (uint32_t i = kk + threadIdx.x; i < npad; i += blockDim.x)
+		comp[i] = ~0ull;
+	block_bitonic_sort(comp, pay, npad);
+	for (uint32_t i = threadIdx.x; i < kk; i += blockDim.x)
+		picked[(size_t) q * k + i] = (uint32_t) comp[i];
+}
+
+/* a wave per (query, picked block): lane l sums 16-byte pieces of row l % 32 against the query's, halves joined at the end */
+__global__ __launch_bounds__(256) void
+k_i8_rescore(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, I8Out o, uint32_t k,
+			 const uint32_t *__restrict__ picked, const uint32_t *__restrict__ npicked, float *__restrict__ cand)
+{
+	const int	lane = threadIdx.x & 63;
+	const uint32_t slot = blockIdx.x * 4 + (threadIdx.x >> 6);
+	const uint32_t q = blockIdx.y;
+
+	if (slot >= npicked[q])
+		return;
+	const uint32_t rb = picked[(size_t) q * k + slot];
+	const unsigned char *a = rows + (size_t) rb * 32u * kp + lane * 16;
+	const unsigned char *b = queries + (size_t) (q >> 5) * 32u * kp + (q & 31) * 16 + (lane >> 5) * 512;
+	int			s = 0;
+
+	for (uint32_t e = 0; e < kp; e += 32)
+	{
+		const i8_v4i x = *(const i8_v4i *) (a + (size_t) e * 32);
+		const i8_v4i y = *(const i8_v4i *) (b + (size_t) e * 32);
+
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+			s = __builtin_amdgcn_sdot4(x[i], y[i], s, false);
+	}
+	s += __shfl_xor(s, 32, 64);
+	if (lane < 32)
+	{
+		const uint32_t r = rb * 32 + lane;
+		float		v = i8_score(s, o.rscale[r], o.qscale[q]);
+
+		if (o.bias && r < o.n)
+			v = v + o.bias[r];
+		if (!(v > I8_NINF) || (o.mask && !(o.mask[(int64_t) q * o.mask_stride + rb] >> lane & 1u)))
+			v = I8_NINF;
+		cand[((size_t) q * k + slot) * 32 + lane] = v + 0.0f;	/* (-0 and 0 are equal scores) */
+	}
+}
+
+/* the k best of a query's candidates, which lie in the order of their ids */
+__global__ __launch_bounds__(256) void
+k_i8_best(const float *__restrict__ cand, const uint32_t *__restrict__ picked, const uint32_t *__restrict__ npicked, uint32_t k,
+		  int64_t *__restrict__ ids, float *__restrict__ scores)
+{
+	__shared__ uint32_t hist[256], sh[16];
+	__shared__ uint64_t comp[NDBHIP_MAX_K];
+	__shared__ uint32_t pay[NDBHIP_MAX_K];
+	const uint32_t q = blockIdx.x;
+	const float *c = cand + (size_t) q * k * 32;
+	const uint32_t n = npicked[q] * 32;
+	auto		f = [&](uint32_t i, uint32_t &bits) -> bool {
+		const float m = c[i];
+
+		bits = __float_as_uint(-m);
+		return m > I8_NINF;
+	};
+	uint32_t	T, less, kk, eq;
+
+	block_radix_select(f, n, k, hist, sh, T, less, kk, eq);
+	if (kk > 0)
+	{
+		block_ordered_gather(f, n, T, kk - less, sh, [&](int cls, uint32_t rank, uint32_t i, uint32_t bits) {
+			comp[cls == 0 ? rank : less + rank] = (uint64_t) ndb_key_from_bits(bits) << 32 | i;
+		});
+		__syncthreads();
+		uint32_t	npad = 1;
+
+		while (npad < kk)
+			npad <<= 1;
+		for (uint32_t i = kk + threadIdx.x; i < npad; i += blockDim.x)
+			comp[i] = ~0ull;
+		block_bitonic_sort(comp, pay, npad);
+	}
+	for (uint32_t i = threadIdx.x; i < k; i += blockDim.x)
+	{
+		int64_t		id = -1;
+		float		s = I8_NINF;
+
+		if (i < kk)
+		{
+			const uint32_t at = (uint32_t) comp[i];
+
+			id = (int64_t) picked[(size_t) q * k + at / 32] * 32 + at % 32;
+			s = c[at];
+		}
+		ids[(size_t) q * k + i] = id;
+		scores[(size_t) q * k + i] = s;
+	}
+}
+
+__global__ __launch_bounds__(256) void
+k_i8_none(int64_t *__restrict__ ids, float *__restrict__ scores, uint64_t n)
+{
+	const uint64_t i = (uint64_t) blockIdx.x * 256 + threadIdx.x;
+
+	if (i < n)
+	{
+		ids[i] = -1;
+		scores[i] = I8_NINF;
+	}
+}
+
+/* ================================================================== */
+/* scores: penalties, biases, masks                                    */
+/* ================================================================== */
+
+/*
+ * A block of threads takes COLS columns of one query: counts how often the query's list names each of them (the whole
+ * list is read per block: it is short next to the columns, and LDS counters need neither a sort nor a hash nor a bound
+ * on its length), then passes over the scores once.  Bound by HBM: a score read and written, a bit of mask.
+ */
+template <class T>
+__global__ __launch_bounds__(256) void
+k_scores_adjust(const T *scores, int64_t stride, int64_t n, int cols, int svec, const int64_t *__restrict__ seen_off,
+				const int32_t *__restrict__ seen_ids, const float *__restrict__ penalties, const float *__restrict__ bias, int64_t bias_stride,
+				const uint32_t *__restrict__ mask, int64_t mask_stride, T *out, int64_t ostride, int q0)
+{
+	constexpr int VEC = 16 / sizeof(T);
+	extern __shared__ uint32_t cnt[];
+	const int64_t q = q0 + blockIdx.y;
+	const int64_t c0 = (int64_t) blockIdx.x * cols;
+	const int	m = (int) min((int64_t) cols, n - c0);
+	const int64_t lo = seen_off ? seen_off[q] : 0, hi = seen_off ? seen_off[q + 1] : 0;
+	const bool	seen = hi > lo;
+	float		repeat = 1.0f, presence = 0.0f, frequency = 0.0f;
+
+	if (seen)
+	{
+		repeat = penalties[3 * q];
+		presence = penalties[3 * q + 1];
+		frequency = penalties[3 * q + 2];
+		for (int i = threadIdx.x; i < m; i += 256)
+			cnt[i] = 0;
+		__syncthreads();
+		for (int64_t i = lo + threadIdx.x; i < hi; i += 256)
+		{
+			const int64_t at = (int64_t) seen_ids[i] - c0;
+
+			if (at >= 0 && at < m)
+				atomicAdd(&cnt[at], 1u);
+		}
+		__syncthreads();
+	}
+	const T    *src = scores + q * stride + c0;
+	T		   *dst = out + q * ostride + c0;
+	const float *bv = bias ? bias + q * bias_stride + c0 : nullptr;
+	const uint32_t *mv = mask ? mask + q * mask_stride + c0 / 32 : nullptr;
+
+	for (int e = threadIdx.x * VEC; e < m; e += 256 * VEC)
+	{
+		I8Vec<T, VEC> v;
+		const bool	whole = svec && e + VEC <= m;
+		const uint32_t word = mv ? mv[e / 32] >> (e % 32) : 0xFFFFFFFFu;
+
+		if (whole)
+			v = *(const I8Vec<T, VEC> *) (src + e);
+		else
+#pragma unroll
+			for (int i = 0; i < VEC; i++)
+				if (e + i < m)
+					v.v[i] = src[e + i];
+#pragma unroll
+		for (int i = 0; i < VEC; i++)
+			if (e + i < m)
+			{
+				float		s = I8Elem<T>::load(v.v[i]);
+				const uint32_t c = seen ? cnt[e + i] : 0u;
+
+				if (c > 0)
+				{
+					s = s > 0.0f ? s / repeat : s * repeat;
+					s = s - (presence + (float) c * frequency);
+				}
+				if (bv)
+					s = s + bv[e + i];
+				if (!(word >> i & 1u))
+					s = I8_NINF;
+				v.v[i] = I8Elem<T>::store(s);
+			}
+		if (whole)
+			*(I8Vec<T, VEC> *) (dst + e) = v;
+		else
+#pragma unroll
+			for (int i = 0; i < VEC; i++)
+				if (e + i < m)
+					dst[e + i] = v.v[i];
+	}
+}
+
+/* ================================================================== */
+/* host                                                                */
+/* ================================================================== */
+
+struct ndbhip_i8
+{
+	int			dim = 0;
+	uint32_t	kp = 0;			/* dimensions, padded */
+	int64_t		n = 0;			/* rows */
+	int64_t		np = 0;			/* rows laid out */
+	unsigned char *d_codes = nullptr;
+	float	   *d_scales = nullptr;
+};
+
+#define I8_MAX_DIM	32767
+#define I8_MAX_ROWS	((int64_t) 0x7FFFFF00)
+
+static int
+i8_type_size(int dtype)
+{
+	return dtype == NDBHIP_F32 ? 4 : dtype == NDBHIP_F16 || dtype == NDBHIP_BF16 ? 2 : dtype == NDBHIP_I8 ? 1 : 0;
+}
+
+static bool
+i8_aligned(const void *p, int64_t stride_bytes, unsigned to)
+{
+	return ((uintptr_t) p % to) == 0 && (stride_bytes % to) == 0;
+}
+
+/* lanes for a row of `units` lane-loads, as a power of two's exponent: the smallest that covers it, at most a wave */
+static int
+i8_lanes_log2(int64_t units)
+{
+	int			l = 0;
+
+	while (l < 6 && (1 << l) < units)
+		l++;
+	return l;
+}
+
+/* rows a launch takes: HIP counts a grid's threads in 32 bits, and a thread of these kernels takes at least four bytes of a row */
+static int64_t
+i8_slab_rows(int dim)
+{
+	return std::max<int64_t>(I8_ROW_PAD, ((int64_t) 1 << 30) / i8_up((uint32_t) dim, I8_DIM_PAD) / I8_ROW_PAD * I8_ROW_PAD);
+}
+
+template <class T, bool BLOCKED>
+static int
+i8_quantize_launch(const void *d_x, int64_t nrows, int64_t nrows_out, int dim, int64_t xstride, unsigned char *codes, int64_t cstride,
+				   uint32_t kp, float *scales)
+{
+	constexpr int VEC = 16 / sizeof(T);
+	const int	ll = i8_lanes_log2((dim + VEC - 1) / VEC);
+	const int	xvec = i8_aligned(d_x, xstride * (int64_t) sizeof(T), 16);
+	const int	cvec = i8_aligned(codes, cstride, VEC);
+	const int64_t slab = i8_slab_rows(dim);
+
+	for (int64_t r0 = 0; r0 < nrows_out; r0 += slab)
+	{
+		const int64_t m = std::min(slab, nrows_out - r0), real = std::max<int64_t>(0, std::min(m, nrows - r0));
+
+		/* (a launch of padding rows alone reads nothing; its pointer stays at the first row) */
+		hipLaunchKernelGGL((k_i8_quantize<T, BLOCKED, 4>), dim3((unsigned) ((m + (256 >> ll) - 1) / (256 >> ll))), dim3(256), 0, g.stream,
+						   (const T *) d_x + (real ? r0 * xstride : 0), real, m, dim, xstride, ll, xvec,
+						   codes + r0 * (BLOCKED ? (int64_t) kp : cstride), cstride, cvec, kp, scales + r0);
+	}
+	HIP_TRY(hipGetLastError());
+	return NDBHIP_OK;
+}
+
+/* rows of any input type -> block layout (or rows of bytes) */
+template <bool BLOCKED>
+static int
+i8_quantize_any(const void *d_x, int dtype, int64_t nrows, int64_t nrows_out, int dim, int64_t xstride, unsigned char *codes, int64_t cstride,
+				uint32_t kp, float *scales)
+{
+	if (dtype == NDBHIP_F32)
+		return i8_quantize_launch<float, BLOCKED>(d_x, nrows, nrows_out, dim, xstride, codes, cstride, kp, scales);
+	if (dtype == NDBHIP_F16)
+		return i8_quantize_launch<__half, BLOCKED>(d_x, nrows, nrows_out, dim, xstride, codes, cstride, kp, scales);
+	return i8_quantize_launch<__hip_bfloat16, BLOCKED>(d_x, nrows, nrows_out, dim, xstride, codes, cstride, kp, scales);
+}
+
+static int
+i8_pack(const void *codes, int64_t stride, const float *scales, int64_t nrows, int64_t nrows_out, int dim, uint32_t kp, unsigned char *dst,
+		float *sout)
+{
+	const int64_t slab = i8_slab_rows(dim);
+
+	for (int64_t r0 = 0; r0 < nrows_out; r0 += slab)
+	{
+		const int64_t m = std::min(slab, nrows_out - r0), real = std::max<int64_t>(0, std::min(m, nrows - r0));
+		const uint64_t units = (uint64_t) m * (kp / 16);
+
+		hipLaunchKernelGGL(k_i8_blocks<true>, dim3((unsigned) ((units + 255) / 256)), dim3(256), 0, g.stream,
+						   (const unsigned char *) codes + (real ? r0 * stride : 0), dst + r0 * kp, stride, (int) i8_aligned(codes, stride, 16),
+						   real, m, dim, kp, scales + (real ? r0 : 0), sout + r0);
+	}
+	HIP_TRY(hipGetLastError());
+	return NDBHIP_OK;
+}
+
+extern "C" int
+ndbhip_i8_quantize_device(const void *d_x, int dtype, int64_t nrows, int dim, int64_t x_stride, int8_t *d_codes, int64_t codes_stride,
+						  float *d_scales)
+{
+	if (dtype != NDBHIP_F32 && dtype != NDBHIP_F16 && dtype != NDBHIP_BF16)
+		return fail(NDBHIP_ERR_INVALID, "rows to quantise must be NDBHIP_F32, _F16 or _BF16");
+	if (nrows < 0 || nrows > I8_MAX_ROWS || dim < 1 || dim > I8_MAX_DIM || x_stride < dim || codes_stride < dim)
+		return fail(NDBHIP_ERR_INVALID, "bad sizes");
+	if (nrows > 0 && (!d_x || !d_codes || !d_scales))
+		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (nrows == 0)
+		return NDBHIP_OK;
+	return i8_quantize_any<false>(d_x, dtype, nrows, nrows, dim, x_stride, (unsigned char *) d_codes, codes_stride, 0, d_scales);
+}
+
+template <class T>
+static void
+i8_dequantize_launch(const int8_t *codes, int64_t cstride, const float *scales, int64_t nrows, int dim, void *out, int64_t ostride)
+{
+	const int	ll = i8_lanes_log2((dim + 3) / 4);
+	const int64_t per = 256 >> ll, slab = i8_slab_rows(dim);
+
+	for (int64_t r0 = 0; r0 < nrows; r0 += slab)
+	{
+		const int64_t m = std::min(slab, nrows - r0);
+
+		hipLaunchKernelGGL(k_i8_dequantize<T>, dim3((unsigned) ((m + per - 1) / per)), dim3(256), 0, g.stream, codes + r0 * cstride, cstride,
+						   (int) i8_aligned(codes, cstride, 4), scales + r0, m, dim, ll, (T *) out + r0 * ostride, ostride,
+						   (int) i8_aligned(out, ostride * (int64_t) sizeof(T), 4 * sizeof(T)));
+	}
+}
+
+extern "C" int
+ndbhip_i8_dequantize_device(const int8_t *d_codes, int64_t codes_stride, const float *d_scales, int64_t nrows, int dim, void *d_out,
+							int dtype, int64_t out_stride)
+{
+	if (dtype != NDBHIP_F32 && dtype != NDBHIP_F16 && dtype != NDBHIP_BF16)
+		return fail(NDBHIP_ERR_INVALID, "values must be NDBHIP_F32, _F16 or _BF16");
+	if (nrows < 0 || nrows > I8_MAX_ROWS || dim < 1 || dim > I8_MAX_DIM || codes_stride < dim || out_stride < dim)
+		return fail(NDBHIP_ERR_INVALID, "bad sizes");
+	if (nrows > 0 && (!d_codes || !d_scales || !d_out))
+		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (nrows == 0)
+		return NDBHIP_OK;
+	if (dtype == NDBHIP_F32)
+		i8_dequantize_launch<float>(d_codes, codes_stride, d_scales, nrows, dim, d_out, out_stride);
+	else if (dtype == NDBHIP_F16)
+		i8_dequantize_launch<__half>(d_codes, codes_stride, d_scales, nrows, dim, d_out, out_stride);
+	else
+		i8_dequantize_launch<__hip_bfloat16>(d_codes, codes_stride, d_scales, nrows, dim, d_out, out_stride);
+	HIP_TRY(hipGetLastError());
+	return NDBHIP_OK;
+}
+
+extern "C" int
+ndbhip_i8_create(int dim, ndbhip_i8 **out)
+{
+	if (!out)
+		return fail(NDBHIP_ERR_INVALID, "out is NULL");
+	if (dim < 1 || dim > I8_MAX_DIM)
+		return fail(NDBHIP_ERR_INVALID, "dim must be 1 .. %d", I8_MAX_DIM);
+	ndbhip_i8  *t = new (std::nothrow) ndbhip_i8();
+
+	if (!t)
+		return fail(NDBHIP_ERR_NOMEM, "out of host memory");
+	t->dim = dim;
+	t->kp = i8_up((uint32_t) dim, I8_DIM_PAD);
+	*out = t;
+	return NDBHIP_OK;
+}
+
+static int
+i8_clear(ndbhip_i8 *t)
+{
+	unsigned char *c = t->d_codes;
+	float	   *s = t->d_scales;
+
+	t->d_codes = nullptr;
+	t->d_scales = nullptr;
+	t->n = t->np = 0;
+	if (c)
+		HIP_TRY(hipFree(c));
+	if (s)
+		HIP_TRY(hipFree(s));
+	return NDBHIP_OK;
+}
+
+extern "C" int
+ndbhip_i8_destroy(ndbhip_i8 *t)
+{
+	if (!t)
+		return NDBHIP_OK;
+	if (t->d_codes && need_init())
+		return NDBHIP_ERR_NODEVICE;
+	const int	rc = i8_clear(t);
+
+	delete t;
+	return rc;
+}
+
+/* room for `nrows` rows in place of what the table holds */
+static int
+i8_room(ndbhip_i8 *t, int64_t nrows)
+{
+	if (i8_clear(t))
+		return NDBHIP_ERR_HIP;
+	if (nrows == 0)
+		return NDBHIP_OK;
+	const int64_t np = (nrows + I8_ROW_PAD - 1) / I8_ROW_PAD * I8_ROW_PAD;
+	hipError_t	e = hipMalloc((void **) &t->d_codes, (size_t) np * t->kp);
+
+	if (e == hipSuccess)
+		e = hipMalloc((void **) &t->d_scales, (size_t) np * sizeof(float));
+	if (e != hipSuccess)
+	{
+		(void) hipGetLastError();
+		(void) i8_clear(t);
+		return fail(e == hipErrorOutOfMemory ? NDBHIP_ERR_NOMEM : NDBHIP_ERR_HIP, "no room for %lld rows: %s", (long long) nrows,
+					hipGetErrorString(e));
+	}
+	t->np = np;
+	return NDBHIP_OK;
+}
+
+extern "C" int
+ndbhip_i8_load_device(ndbhip_i8 *t, const void *d_rows, int dtype, int64_t nrows, int64_t row_stride, const float *d_scales)
+{
+	if (!t)
+		return fail(NDBHIP_ERR_INVALID, "table is NULL");
+	if (i8_type_size(dtype) == 0)
+		return fail(NDBHIP_ERR_INVALID, "rows must be NDBHIP_F32, _F16, _BF16 or _I8");
+	if (nrows < 0 || nrows > I8_MAX_ROWS || row_stride < t->dim)
+		return fail(NDBHIP_ERR_INVALID, "bad sizes");
+	if (nrows > 0 && (!d_rows || (dtype == NDBHIP_I8) != (d_scales != nullptr)))
+		return fail(NDBHIP_ERR_INVALID, "rows are NULL, or scales given for rows that are not NDBHIP_I8 (or none for rows that are)");
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	int			rc = i8_room(t, nrows);
+
+	if (rc || nrows == 0)
+		return rc;
+	if (dtype == NDBHIP_I8)
+		rc = i8_pack(d_rows, row_stride, d_scales, nrows, t->np, t->dim, t->kp, t->d_codes, t->d_scales);
+	else
+		rc = i8_quantize_any<true>(d_rows, dtype, nrows, t->np, t->dim, row_stride, t->d_codes, 0, t->kp, t->d_scales);
+	/* (the rows may go once this returns, and the table may be read on any stream) */
+	if (!rc && hipStreamSynchronize(g.stream) != hipSuccess)
+		rc = fail(NDBHIP_ERR_HIP, "loading an 8-bit table failed");
+	if (rc)
+		(void) i8_clear(t);
+	else
+		t->n = nrows;
+	return rc;
+}
+
+extern "C" int
+ndbhip_i8_load(ndbhip_i8 *t, const float *rows, int64_t nrows)
+{
+	if (!t)
+		return fail(NDBHIP_ERR_INVALID, "table is NULL");
+	if (nrows < 0 || nrows > I8_MAX_ROWS || (nrows > 0 && !rows))
+		return fail(NDBHIP_ERR_INVALID, "bad arguments");
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	int			rc = i8_room(t, nrows);
+
+	if (rc || nrows == 0)
+		return rc;
+	/* through a device buffer of whole row blocks, so that a table larger than the free memory's half still loads */
+	const int64_t slab = std::min<int64_t>(t->np, std::max<int64_t>(I8_ROW_PAD, ((int64_t) 256 << 20) / (4 * t->dim) / I8_ROW_PAD * I8_ROW_PAD));
+	float	   *d = nullptr;
+
+	if (hipMalloc((void **) &d, (size_t) std::min(slab, nrows) * t->dim * sizeof(float)) != hipSuccess)
+	{
+		(void) hipGetLastError();
+		(void) i8_clear(t);
+		return fail(NDBHIP_ERR_NOMEM, "no room to load through");
+	}
+	for (int64_t r0 = 0; r0 < nrows && !rc; r0 += slab)
+	{
+		const int64_t m = std::min(slab, nrows - r0), mp = std::min(slab, t->np - r0);
+
+		if (hipMemcpyAsync(d, rows + r0 * t->dim, (size_t) m * t->dim * sizeof(float), hipMemcpyHostToDevice, g.stream) != hipSuccess)
+			rc = fail(NDBHIP_ERR_HIP, "loading an 8-bit table failed");
+		else
+			rc = i8_quantize_any<true>(d, NDBHIP_F32, m, mp, t->dim, t->dim, t->d_codes + (size_t) r0 * t->kp, 0, t->kp, t->d_scales + r0);
+	}
+	if (hipStreamSynchronize(g.stream) != hipSuccess && !rc)
+		rc = fail(NDBHIP_ERR_HIP, "loading an 8-bit table failed");
+	(void) hipFree(d);
+	if (rc)
+		(void) i8_clear(t);
+	else
+		t->n = nrows;
+	return rc;
+}
+
+extern "C" int
+ndbhip_i8_export_device(const ndbhip_i8 *t, int8_t *d_codes, int64_t codes_stride, float *d_scales)
+{
+	if (!t)
+		return fail(NDBHIP_ERR_INVALID, "table is NULL");
+	if (t->n > 0 && (!d_codes || !d_scales || codes_stride < t->dim))
+		return fail(NDBHIP_ERR_INVALID, "bad arguments");
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (t->n == 0)
+		return NDBHIP_OK;
+	const int64_t slab = i8_slab_rows(t->dim);
+
+	for (int64_t r0 = 0; r0 < t->n; r0 += slab)
+	{
+		const int64_t m = std::min(slab, t->n - r0);
+		const uint64_t units = (uint64_t) m * (t->kp / 16);
+
+		hipLaunchKernelGGL(k_i8_blocks<false>, dim3((unsigned) ((units + 255) / 256)), dim3(256), 0, g.stream,
+						   (const unsigned char *) t->d_codes + r0 * t->kp, (unsigned char *) d_codes + r0 * codes_stride, codes_stride,
+						   (int) i8_aligned(d_codes, codes_stride, 16), m, m, t->dim, t->kp, t->d_scales + r0, d_scales + r0);
+	}
+	HIP_TRY(hipGetLastError());
+	return NDBHIP_OK;
+}
+
+extern "C" int64_t
+ndbhip_i8_nrows(const ndbhip_i8 *t)
+{
+	return t ? t->n : -1;
+}
+
+extern "C" int
+ndbhip_i8_dim(const ndbhip_i8 *t)
+{
+	return t ? t->dim : -1;
+}
+
+/* ------------------------------------------------------------------ */
+
+static size_t
+i8_round(size_t b)
+{
+	return (b + 255) & ~(size_t) 255;
+}
+
+/* workspace of a batch of nq queries: their blocks and scales, then what a search leaves between its kernels */
+struct I8Ws
+{
+	uint32_t	nqp, ng, ngp;
+	size_t		q_off, qs_off, gm_off, pick_off, npick_off, cand_off, total;
+};
+
+static I8Ws
+i8_ws(const ndbhip_i8 *t, int nq, int k)
+{
+	I8Ws		w;
+	size_t		at = 0;
+	auto		take = [&](size_t b) { const size_t o = at; at += i8_round(b); return o; };
+
+	w.nqp = i8_up((uint32_t) nq, I8_ROW_PAD);
+	w.ng = (uint32_t) ((t->n + 31) / 32);
+	w.ngp = i8_up(w.ng, 8);
+	w.q_off = take((size_t) w.nqp * t->kp);
+	w.qs_off = take((size_t) w.nqp * sizeof(float));
+	w.gm_off = take(k ? (size_t) nq * w.ngp * sizeof(float) : 0);
+	w.pick_off = take((size_t) nq * k * sizeof(uint32_t));
+	w.npick_off = take(k ? (size_t) nq * sizeof(uint32_t) : 0);
+	w.cand_off = take((size_t) nq * k * 32 * sizeof(float));
+	w.total = at;
+	return w;
+}
+
+/* queries a search takes at a time: as many as leave its workspace near a gigabyte, in whole tiles */
+static int
+i8_chunk(const ndbhip_i8 *t, int nq, int k)
+{
+	const size_t per = (size_t) t->kp + (size_t) (t->n + 255) / 8 + (size_t) k * 132 + 8;
+	const int64_t m = std::max<int64_t>(256, (int64_t) (((size_t) 1 << 30) / per) / 256 * 256);
+
+	return (int) std::min<int64_t>(nq, std::min<int64_t>(m, 4096));
+}
+
+extern "C" int
+ndbhip_i8_workspace(const ndbhip_i8 *t, int nq, int k, size_t *bytes)
+{
+	if (!t || !bytes)
+		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
+	if (nq < 0 || k < 0 || k > NDBHIP_MAX_K)
+		return fail(NDBHIP_ERR_INVALID, "bad sizes");
+	*bytes = nq == 0 || t->n == 0 ? 0 : i8_ws(t, i8_chunk(t, nq, k), k).total;
+	return NDBHIP_OK;
+}
+
+static int
+i8_check_queries(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_q_scales, int nq, int64_t q_stride)
+{
+	if (!t)
+		return fail(NDBHIP_ERR_INVALID, "table is NULL");
+	if (i8_type_size(q_type) == 0)
+		return fail(NDBHIP_ERR_INVALID, "queries must be NDBHIP_F32, _F16, _BF16 or _I8");
+	if (nq < 0 || q_stride < t->dim)
+		return fail(NDBHIP_ERR_INVALID, "bad sizes");
+	if (nq > 0 && (!d_q || (q_type == NDBHIP_I8) != (d_q_scales != nullptr)))
+		return fail(NDBHIP_ERR_INVALID, "queries are NULL, or scales given for queries that are not NDBHIP_I8 (or none for queries that are)");
+	return NDBHIP_OK;
+}
+
+static int
+i8_check_ws(const ndbhip_i8 *t, int nq, int k, const void *d_ws, size_t ws_bytes)
+{
+	const size_t want = i8_ws(t, i8_chunk(t, nq, k), k).total;
+
+	if (!d_ws || ws_bytes < want || ((uintptr_t) d_ws & 255))
+		return fail(NDBHIP_ERR_INVALID, "the workspace must be %zu bytes on a 256-byte boundary (ndbhip_i8_workspace)", want);
+	return NDBHIP_OK;
+}
+
+/* a batch's queries into the workspace, as bytes in the block layout */
+static int
+i8_take_queries(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_q_scales, int64_t q0, int m, int64_t q_stride, char *ws,
+				const I8Ws &w)
+{
+	const char *q = (const char *) d_q + q0 * q_stride * i8_type_size(q_type);
+	unsigned char *codes = (unsigned char *) ws + w.q_off;
+	float	   *scales = (float *) (ws + w.qs_off);
+
+	if (q_type == NDBHIP_I8)
+		return i8_pack(q, q_stride, d_q_scales + q0, m, w.nqp, t->dim, t->kp, codes, scales);
+	return i8_quantize_any<true>(q, q_type, m, w.nqp, t->dim, q_stride, codes, 0, t->kp, scales);
+}
+
+template <int MODE, class T>
+static int
+i8_multiply(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
+{
+	const uint32_t nrb = (o.n + 31) / 32, nqb = (o.nq + 31) / 32;
+
+	hipLaunchKernelGGL((k_i8_stream<2, MODE, T>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
+					   nrb, nqb, o);
+	HIP_TRY(hipGetLastError());
+	return NDBHIP_OK;
+}
+
+extern "C" int
+ndbhip_i8_product_device(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_q_scales, int nq, int64_t q_stride,
+						 const float *d_bias, void *d_out, int out_type, int64_t out_stride, void *d_ws, size_t ws_bytes)
+{
+	int			rc = i8_check_queries(t, d_q, q_type, d_q_scales, nq, q_stride);
+
+	if (rc)
+		return rc;
+	if (out_type != NDBHIP_F32 && out_type != NDBHIP_F16 && out_type != NDBHIP_BF16)
+		return fail(NDBHIP_ERR_INVALID, "scores must be NDBHIP_F32, _F16 or _BF16");
+	if (out_stride < t->n)
+		return fail(NDBHIP_ERR_INVALID, "out_stride is smaller than the table's rows");
+	if (nq > 0 && t->n > 0 && !d_out)
+		return fail(NDBHIP_ERR_INVALID, "out is NULL");
+	if (nq > 0 && t->n > 0 && (rc = i8_check_ws(t, nq, 0, d_ws, ws_bytes)))
+		return rc;
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (nq == 0 || t->n == 0)
+		return NDBHIP_OK;
+	const int	chunk = i8_chunk(t, nq, 0);
+	const int	osz = i8_type_size(out_type);
+
+	for (int64_t q0 = 0; q0 < nq; q0 += chunk)
+	{
+		const int	m = (int) std::min<int64_t>(chunk, nq - q0);
+		const I8Ws	w = i8_ws(t, m, 0);
+		I8Out		o = {};
+
+		if ((rc = i8_take_queries(t, d_q, q_type, d_q_scales, q0, m, q_stride, (char *) d_ws, w)))
+			return rc;
+		o.rscale = t->d_scales;
+		o.qscale = (const float *) ((char *) d_ws + w.qs_off);
+		o.bias = d_bias;
+		o.out = (char *) d_out + q0 * out_stride * osz;
+		o.ostride = out_stride;
+		o.ovec = i8_aligned(d_out, out_stride * osz, 4 * osz);
+		o.n = (uint32_t) t->n;
+		o.nq = (uint32_t) m;
+		const unsigned char *qc = (const unsigned char *) d_ws + w.q_off;
+
+		rc = out_type == NDBHIP_F32 ? i8_multiply<0, float>(t, qc, o) : out_type == NDBHIP_F16 ? i8_multiply<0, __half>(t, qc, o) :
+			i8_multiply<0, __hip_bfloat16>(t, qc, o);
+		if (rc)
+			return rc;
+	}
+	NDB_STAT_ADD(queries, nq);
+	__atomic_fetch_add(&g.host_rows, (uint64_t) nq * t->n, __ATOMIC_RELAXED);
+	__atomic_fetch_add(&g.host_bytes, (uint64_t) nq * t->n * t->dim, __ATOMIC_RELAXED);
+	return NDBHIP_OK;
+}
+
+extern "C" int
+ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_q_scales, int nq, int64_t q_stride,
+						const float *d_bias, const uint32_t *d_mask, int64_t mask_stride, int k, int64_t *d_ids, float *d_scores,
+						void *d_ws, size_t ws_bytes)
+{
+	int			rc = i8_check_queries(t, d_q, q_type, d_q_scales, nq, q_stride);
+
+	if (rc)
+		return rc;
+	if (k < 1 || k > NDBHIP_MAX_K)
+		return fail(NDBHIP_ERR_INVALID, "k must be 1 .. %d", NDBHIP_MAX_K);
+	if (d_mask && mask_stride != 0 && mask_stride < (t->n + 31) / 32)
+		return fail(NDBHIP_ERR_INVALID, "mask_stride must be 0 (one mask) or at least a word for every 32 rows");
+	if (nq > 0 && (!d_ids || !d_scores))
+		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
+	if (nq > 0 && t->n > 0 && (rc = i8_check_ws(t, nq, k, d_ws, ws_bytes)))
+		return rc;
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (nq == 0)
+		return NDBHIP_OK;
+	if (t->n == 0)
+	{
+		const uint64_t m = (uint64_t) nq * k;
+
+		hipLaunchKernelGGL(k_i8_none, dim3((unsigned) ((m + 255) / 256)), dim3(256), 0, g.stream, d_ids, d_scores, m);
+		HIP_TRY(hipGetLastError());
+		return NDBHIP_OK;
+	}
+	const int	chunk = i8_chunk(t, nq, k);
+
+	for (int64_t q0 = 0; q0 < nq; q0 += chunk)
+	{
+		const int	m = (int) std::min<int64_t>(chunk, nq - q0);
+		const I8Ws	w = i8_ws(t, m, k);
+		char	   *ws = (char *) d_ws;
+		const unsigned char *qc = (const unsigned char *) ws + w.q_off;
+		uint32_t   *picked = (uint32_t *) (ws + w.pick_off), *npicked = (uint32_t *) (ws + w.npick_off);
+		float	   *cand = (float *) (ws + w.cand_off);
+		I8Out		o = {};
+
+		if ((rc = i8_take_queries(t, d_q, q_type, d_q_scales, q0, m, q_stride, ws, w)))
+			return rc;
+		o.rscale = t->d_scales;
+		o.qscale = (const float *) (ws + w.qs_off);
+		o.bias = d_bias;
+		o.mask = d_mask ? d_mask + q0 * mask_stride : nullptr;
+		o.mask_stride = mask_stride;
+		o.gmax = (float *) (ws + w.gm_off);
+		o.ngp = w.ngp;
+		o.n = (uint32_t) t->n;
+		o.nq = (uint32_t) m;
+		if ((rc = i8_multiply<1, float>(t, qc, o)))
+			return rc;
+		hipLaunchKernelGGL(k_i8_pick, dim3(m), dim3(256), 0, g.stream, o.gmax, w.ngp, w.ng, (uint32_t) k, picked, npicked);
+		hipLaunchKernelGGL(k_i8_rescore, dim3((k + 3) / 4, m), dim3(256), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, picked,
+						   npicked, cand);
+		hipLaunchKernelGGL(k_i8_best, dim3(m), dim3(256), 0, g.stream, cand, picked, npicked, (uint32_t) k, d_ids + q0 * k,
+						   d_scores + q0 * k);
+		HIP_TRY(hipGetLastError());
+	}
+	NDB_STAT_ADD(queries, nq);
+	__atomic_fetch_add(&g.host_rows, (uint64_t) nq * t->n, __ATOMIC_RELAXED);
+	__atomic_fetch_add(&g.host_bytes, (uint64_t) nq * t->n * t->dim, __ATOMIC_RELAXED);
+	return NDBHIP_OK;
+}
+
+/* host queries in, host results out: the shape of ndbhip_ivf_search */
+extern "C" int
+ndbhip_i8_search(const ndbhip_i8 *t, const float *queries, int nq, const float *bias, const uint32_t *mask, int64_t mask_stride, int k,
+				 int64_t *ids, float *scores)
+{
+	if (!t)
+		return fail(NDBHIP_ERR_INVALID, "table is NULL");
+	if (nq < 0 || k < 1 || k > NDBHIP_MAX_K)
+		return fail(NDBHIP_ERR_INVALID, "bad sizes");
+	if (mask && mask_stride != 0 && mask_stride < (t->n + 31) / 32)
+		return fail(NDBHIP_ERR_INVALID, "mask_stride must be 0 (one mask) or at least a word for every 32 rows");
+	if (nq > 0 && (!queries || !ids || !scores))
+		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (nq == 0)
+		return NDBHIP_OK;
+	size_t		wsb = 0;
+	const size_t qb = (size_t) nq * t->dim * sizeof(float), bb = bias ? (size_t) t->n * sizeof(float) : 0;
+	const size_t words = (size_t) (t->n + 31) / 32;
+	const size_t mb = !mask ? 0 : (mask_stride ? (size_t) (nq - 1) * mask_stride + words : words) * sizeof(uint32_t);
+	const size_t ib = (size_t) nq * k * sizeof(int64_t), sb = (size_t) nq * k * sizeof(float);
+	int			rc = ndbhip_i8_workspace(t, nq, k, &wsb);
+
+	if (rc)
+		return rc;
+	char	   *d = nullptr;
+	const size_t total = i8_round(wsb) + i8_round(qb) + i8_round(bb) + i8_round(mb) + i8_round(ib) + i8_round(sb);
+
+	if (hipMalloc((void **) &d, total) != hipSuccess)
+	{
+		(void) hipGetLastError();
+		return fail(NDBHIP_ERR_NOMEM, "no room for a search of %d queries (%zu bytes)", nq, total);
+	}
+	char	   *d_q = d + i8_round(wsb), *d_b = d_q + i8_round(qb), *d_m = d_b + i8_round(bb), *d_i = d_m + i8_round(mb), *d_s = d_i + i8_round(ib);
+	bool		ok = hipMemcpyAsync(d_q, queries, qb, hipMemcpyHostToDevice, g.stream) == hipSuccess;
+
+	if (ok && bb)
+		ok = hipMemcpyAsync(d_b, bias, bb, hipMemcpyHostToDevice, g.stream) == hipSuccess;
+	if (ok && mb)
+		ok = hipMemcpyAsync(d_m, mask, mb, hipMemcpyHostToDevice, g.stream) == hipSuccess;
+	if (!ok)
+		rc = fail(NDBHIP_ERR_HIP, "copying the queries failed");
+	if (!rc)
+		rc = ndbhip_i8_search_device(t, d_q, NDBHIP_F32, nullptr, nq, t->dim, bb ? (const float *) d_b : nullptr,
+									 mb ? (const uint32_t *) d_m : nullptr, mask_stride, k, (int64_t *) d_i, (float *) d_s, d, wsb);
+	if (!rc && (hipMemcpyAsync(ids, d_i, ib, hipMemcpyDeviceToHost, g.stream) != hipSuccess ||
+				hipMemcpyAsync(scores, d_s, sb, hipMemcpyDeviceToHost, g.stream) != hipSuccess))
+		rc = fail(NDBHIP_ERR_HIP, "copying the results failed");
+	if (hipStreamSynchronize(g.stream) != hipSuccess && !rc)
+		rc = fail(NDBHIP_ERR_HIP, "the search failed");
+	(void) hipFree(d);
+	return rc;
+}
+
+/* ------------------------------------------------------------------ */
+
+template <class T>
+static void
+scores_adjust_launch(const void *s, int64_t stride, int nq, int64_t n, const int64_t *off, const int32_t *ids, const float *pen, const float *bias,
+					 int64_t bias_stride, const uint32_t *mask, int64_t mask_stride, void *out, int64_t ostride)
+{
+	const int	cols = (int64_t) nq * n >= ((int64_t) 8 << 20) ? 8192 : 2048;
+	const int	vec = i8_aligned(s, stride * (int64_t) sizeof(T), 16) && i8_aligned(out, ostride * (int64_t) sizeof(T), 16);
+
+	for (int q0 = 0; q0 < nq; q0 += 65535)
+		hipLaunchKernelGGL(k_scores_adjust<T>, dim3((unsigned) ((n + cols - 1) / cols), std::min(65535, nq - q0)), dim3(256),
+						   off ? cols * sizeof(uint32_t) : 0, g.stream, (const T *) s, stride, n, cols, vec, off, ids, pen, bias, bias_stride,
+						   mask, mask_stride, (T *) out, ostride, q0);
+}
+
+extern "C" int
+ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, int64_t stride, const int64_t *d_seen_off,
+							const int32_t *d_seen_ids, const float *d_penalties, const float *d_bias, int64_t bias_stride,
+							const uint32_t *d_mask, int64_t mask_stride, void *d_out, int64_t out_stride)
+{
+	if (dtype != NDBHIP_F32 && dtype != NDBHIP_F16 && dtype != NDBHIP_BF16)
+		return fail(NDBHIP_ERR_INVALID, "scores must be NDBHIP_F32, _F16 or _BF16");
+	if (nq < 0 || n < 0 || n > I8_MAX_ROWS || stride < n || out_stride < n)
+		return fail(NDBHIP_ERR_INVALID, "bad sizes");
+	if (d_bias && bias_stride != 0 && bias_stride < n)
+		return fail(NDBHIP_ERR_INVALID, "bias_stride must be 0 (one bias) or at least n");
+	if (d_mask && mask_stride != 0 && mask_stride < (n + 31) / 32)
+		return fail(NDBHIP_ERR_INVALID, "mask_stride must be 0 (one mask) or at least a word for every 32 scores");
+	if (d_seen_off && (!d_seen_ids || !d_penalties))
+		return fail(NDBHIP_ERR_INVALID, "offsets without ids or penalties");
+	if (nq > 0 && n > 0 && (!d_scores || !d_out))
+		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
+	if (nq > 1 && d_scores == d_out && stride != out_stride)
+		return fail(NDBHIP_ERR_INVALID, "in place, the two strides must be the same");
+	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (nq == 0 || n == 0)
+		return NDBHIP_OK;
+	if (dtype == NDBHIP_F32)
+		scores_adjust_launch<float>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, d_penalties, d_bias, bias_stride, d_mask, mask_stride,
+									d_out, out_stride);
+	else if (dtype == NDBHIP_F16)
+		scores_adjust_launch<__half>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, d_penalties, d_bias, bias_stride, d_mask, mask_stride,
+									 d_out, out_stride);
+	else
+		scores_adjust_launch<__hip_bfloat16>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, d_penalties, d_bias, bias_stride, d_mask,
+											 mask_stride, d_out, out_stride);
+	HIP_TRY(hipGetLastError());
+	return NDBHIP_OK;
+}

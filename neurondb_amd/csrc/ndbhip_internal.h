@@ -63,7 +63,12 @@ extern thread_local hipStream_t ndbhip_tl_stream;
 struct StreamRef
 {
 	hipStream_t dflt = nullptr;
-	operator hipStream_t() const { return ndbhip_tl_stream ? ndbhip_tl_stream : dflt; }
+	operator hipStream_t() const
+	{
+		const hipStream_t s = ndbhip_tl_stream ? ndbhip_tl_stream : dflt;
+
+		return s == (hipStream_t) NDBHIP_STREAM_LEGACY ? nullptr : s;
+	}
 	StreamRef &operator=(hipStream_t s) { dflt = s; return *this; }
 };
 

@@ -1,0 +1,338 @@
+"""8-bit tables and scores over the C ABI (include/ndbhip.h, "8-bit tables and scores"): rows as signed bytes with one
+scale each, the int8 product of a batch of queries with a table, penalties / biases / masks over scores, and the k best
+rows of a table.
+
+Everything here takes and returns torch tensors on the device the library runs on, is ordered on torch's current stream
+and can be captured into a graph (the workspace of a call comes from torch's allocator; a graph owns its own).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from ._lib import ERR_INVALID, NdbHipError, check, ensure_init, lib
+
+STREAM_LEGACY = 1           # NDBHIP_STREAM_LEGACY: the default stream, whose own handle is 0
+
+
+def _bad(msg):
+    return NdbHipError(ERR_INVALID, msg)
+
+
+def _types():
+    import torch
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+
+
+class _OnTorchStream:
+    """The library's work of this thread on torch's current stream of the library's device, for the calls inside."""
+
+    def __enter__(self):
+        import torch
+        s = torch.cuda.current_stream(_lib._device).cuda_stream
+        self.prev = C.c_void_p()
+        check(lib().ndbhip_swap_thread_stream(C.c_void_p(s or STREAM_LEGACY), C.byref(self.prev)))
+        return self
+
+    def __exit__(self, *exc):
+        check(lib().ndbhip_swap_thread_stream(self.prev, C.byref(C.c_void_p())))
+        return False
+
+
+def _here():
+    """the library's device, initialised on torch's current one if it is not yet"""
+    import torch
+    if not _lib._inited:
+        ensure_init(torch.cuda.current_device())
+    return torch.device("cuda", _lib._device)
+
+
+def _tensor(t, name, dtypes, ndim, device):
+    """checks what every tensor argument has to be; the last dimension's elements are neighbours"""
+    import torch
+    if not isinstance(t, torch.Tensor):
+        raise _bad(f"{name} must be a torch tensor")
+    if t.device != device:
+        raise _bad(f"{name} is on {t.device}, the library on {device}")
+    if t.dtype not in dtypes:
+        raise _bad(f"{name} must be one of {[str(d) for d in dtypes]}, not {t.dtype}")
+    if t.dim() not in (ndim if isinstance(ndim, tuple) else (ndim,)):
+        raise _bad(f"{name} has {t.dim()} dimensions")
+    return t
+
+
+def _rows(t):
+    """(tensor with neighbouring elements in a row and rows that do not overlap, elements from a row to the next)"""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _out_rows(t, name):
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise _bad(f"{name} must have neighbouring elements in a row and rows that do not overlap")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _p(t):
+    return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def _floats():
+    import torch
+    return (torch.float32, torch.float16, torch.bfloat16)
+
+
+def quantize_rows(x, codes=None, scales=None):
+    """Rows [n, dim] (float32, float16, bfloat16) -> (codes int8 [n, dim], scales float32 [n]); ndbhip_i8_quantize_device."""
+    import torch
+    dev = _here()
+    x, stride = _rows(_tensor(x, "x", _floats(), 2, dev))
+    n, dim = x.shape
+    if codes is None:
+        codes = torch.empty((n, dim), dtype=torch.int8, device=dev)
+    if scales is None:
+        scales = torch.empty(n, dtype=torch.float32, device=dev)
+    _tensor(codes, "codes", (torch.int8,), 2, dev)
+    _tensor(scales, "scales", (torch.float32,), 1, dev)
+    if codes.shape != x.shape or scales.shape != (n,) or not scales.is_contiguous():
+        raise _bad("codes must be [n, dim] and scales [n], contiguous")
+    with _OnTorchStream():
+        check(lib().ndbhip_i8_quantize_device(_p(x), _types()[x.dtype], n, dim, stride, _p(codes), _out_rows(codes, "codes"), _p(scales)))
+    return codes, scales
+
+
+def dequantize_rows(codes, scales, dtype=None, out=None):
+    """The values (codes int8 [n, dim], scales float32 [n]) stand for, as float32 (or `dtype`); ndbhip_i8_dequantize_device."""
+    import torch
+    dev = _here()
+    codes, stride = _rows(_tensor(codes, "codes", (torch.int8,), 2, dev))
+    scales = _tensor(scales, "scales", (torch.float32,), 1, dev).contiguous()
+    if scales.shape[0] != codes.shape[0]:
+        raise _bad("a scale for every row")
+    if out is None:
+        out = torch.empty(codes.shape, dtype=dtype or torch.float32, device=dev)
+    _tensor(out, "out", _floats(), 2, dev)
+    if out.shape != codes.shape or dtype not in (None, out.dtype):
+        raise _bad("out must have the codes' shape and the dtype asked for")
+    with _OnTorchStream():
+        check(lib().ndbhip_i8_dequantize_device(_p(codes), stride, _p(scales), codes.shape[0], codes.shape[1], _p(out),
+                                                _types()[out.dtype], _out_rows(out, "out")))
+    return out
+
+
+def _mask_arg(mask, nq, n, dev):
+    """(tensor, words from one query's mask to the next)"""
+    import torch
+    if mask is None:
+        return None, 0
+    words = {torch.int32} | ({torch.uint32} if hasattr(torch, "uint32") else set())
+    _tensor(mask, "mask", tuple(words), (1, 2), dev)
+    m = mask[None] if mask.dim() == 1 else mask
+    if m.shape[0] not in (1, nq) or m.shape[1] < (n + 31) // 32:
+        raise _bad(f"mask must be [words] or [1 or {nq}, words] with at least {(n + 31) // 32} words of 32 rows")
+    m, stride = _rows(m)
+    return m, 0 if m.shape[0] == 1 else stride
+
+
+def _bias_arg(bias, nq, n, dev, per_query):
+    import torch
+    if bias is None:
+        return None, 0
+    _tensor(bias, "bias", (torch.float32,), (1, 2) if per_query else 1, dev)
+    b = bias[None] if bias.dim() == 1 else bias
+    if b.shape[0] not in (1, nq) or b.shape[1] != n:
+        raise _bad(f"bias must be [{n}]" + (f" or [1 or {nq}, {n}]" if per_query else ""))
+    b, stride = _rows(b)
+    return b, 0 if b.shape[0] == 1 else stride
+
+
+def adjust_scores(scores, seen=None, penalties=None, bias=None, mask=None, out=None):
+    """Penalties, biases and masks over scores [nq, n] (float32, float16, bfloat16); ndbhip_scores_adjust_device.
+
+    seen       (offsets int64 [nq + 1], ids int32 [...]): the ids query q has been given before, an id once for every time
+    penalties  float32 [nq, 3] = repeat, presence, frequency of each query (with `seen`)
+    bias       float32 [n] or [nq, n]
+    mask       int32 words [ceil(n / 32)] or [nq, ceil(n / 32)], bit i % 32 of word i / 32: 0 = -inf
+    out        another tensor of the scores' shape and type, or `scores` itself (in place); None: a new one
+    """
+    import torch
+    dev = _here()
+    _tensor(scores, "scores", _floats(), 2, dev)
+    nq, n = scores.shape
+    if out is not None:
+        _tensor(out, "out", (scores.dtype,), 2, dev)
+        if out.shape != scores.shape:
+            raise _bad("out must have the scores' shape")
+        ostride = _out_rows(out, "out")
+    src, stride = _rows(scores)
+    if out is None:
+        out = torch.empty((nq, n), dtype=scores.dtype, device=dev)
+        ostride = n
+    off = ids = None
+    if (seen is None) != (penalties is None):
+        raise _bad("seen and penalties go together")
+    if seen is not None:
+        off, ids = seen
+        off = _tensor(off, "offsets", (torch.int64,), 1, dev).contiguous()
+        ids = _tensor(ids, "ids", (torch.int32,), 1, dev).contiguous()
+        penalties = _tensor(penalties, "penalties", (torch.float32,), 2, dev).contiguous()
+        if off.shape[0] != nq + 1 or penalties.shape != (nq, 3):
+            raise _bad("offsets must be [nq + 1] and penalties [nq, 3]")
+        if ids.numel() == 0:
+            off = ids = penalties = None
+    bias, bstride = _bias_arg(bias, nq, n, dev, True)
+    mask, mstride = _mask_arg(mask, nq, n, dev)
+    with _OnTorchStream():
+        check(lib().ndbhip_scores_adjust_device(_p(src), _types()[src.dtype], nq, n, stride, _p(off), _p(ids), _p(penalties), _p(bias),
+                                                bstride, _p(mask), mstride, _p(out), ostride))
+    return out
+
+
+class Int8Table:
+    """A table of rows held as signed bytes with one fp32 scale each, resident in HBM (ndbhip_i8).
+
+    Scores are inner products; rows and queries of norm 1 make them cosines, and a bias of -|x|^2 / 2 a row turns the
+    order into the L2 one."""
+
+    def __init__(self, dim: int, device: int | None = None):
+        ensure_init(device)
+        self.dim = int(dim)
+        h = C.c_void_p()
+        check(lib().ndbhip_i8_create(self.dim, C.byref(h)))
+        self._h = h
+
+    def close(self):
+        if getattr(self, "_h", None):
+            check(lib().ndbhip_i8_destroy(self._h))
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def nrows(self) -> int:
+        return int(lib().ndbhip_i8_nrows(self._h))
+
+    def load(self, rows, scales=None):
+        """The table's rows, in place of what it held: a numpy float32 array or a tensor [n, dim] of float32, float16,
+        bfloat16 — quantised on the way — or of int8 with their scales [n]."""
+        import torch
+        if isinstance(rows, np.ndarray):
+            if scales is not None:
+                raise _bad("scales go with int8 tensors")
+            r = np.ascontiguousarray(rows, dtype=np.float32)
+            if r.ndim != 2 or r.shape[1] != self.dim:
+                raise _bad(f"rows must be [n, {self.dim}]")
+            check(lib().ndbhip_i8_load(self._h, r.ctypes.data_as(C.c_void_p), r.shape[0]))
+            return
+        dev = _here()
+        r, stride = _rows(_tensor(rows, "rows", tuple(_types()), 2, dev))
+        if r.shape[1] != self.dim:
+            raise _bad(f"rows must be [n, {self.dim}]")
+        if (r.dtype == torch.int8) != (scales is not None):
+            raise _bad("scales go with int8 rows, and only with them")
+        if scales is not None:
+            scales = _tensor(scales, "scales", (torch.float32,), 1, dev).contiguous()
+            if scales.shape[0] != r.shape[0]:
+                raise _bad("a scale for every row")
+        with _OnTorchStream():
+            check(lib().ndbhip_i8_load_device(self._h, _p(r), _types()[r.dtype], r.shape[0], stride, _p(scales)))
+
+    def export(self):
+        """(codes int8 [n, dim], scales float32 [n])"""
+        import torch
+        dev = _here()
+        n = self.nrows
+        codes = torch.empty((n, self.dim), dtype=torch.int8, device=dev)
+        scales = torch.empty(n, dtype=torch.float32, device=dev)
+        with _OnTorchStream():
+            check(lib().ndbhip_i8_export_device(self._h, _p(codes), self.dim, _p(scales)))
+        return codes, scales
+
+    def _queries(self, queries, dev):
+        import torch
+        scales = None
+        if isinstance(queries, (tuple, list)):
+            queries, scales = queries
+            scales = _tensor(scales, "query scales", (torch.float32,), 1, dev).contiguous()
+        q, stride = _rows(_tensor(queries, "queries", tuple(_types()), 2, dev))
+        if q.shape[1] != self.dim:
+            raise _bad(f"queries must be [nq, {self.dim}]")
+        if (q.dtype == torch.int8) != (scales is not None) or scales is not None and scales.shape[0] != q.shape[0]:
+            raise _bad("int8 queries come as (codes [nq, dim], scales [nq]), others alone")
+        return q, stride, scales
+
+    def _workspace(self, nq, k, dev):
+        import torch
+        b = C.c_size_t(0)
+        check(lib().ndbhip_i8_workspace(self._h, nq, k, C.byref(b)))
+        return torch.empty(max(b.value, 1), dtype=torch.uint8, device=dev), b.value
+
+    def scores(self, queries, bias=None, dtype=None, out=None):
+        """Every score: [nq, nrows] of float32 (or `dtype`, or into `out`); ndbhip_i8_product_device.  queries: [nq, dim] of
+        float32, float16, bfloat16, or (codes, scales)."""
+        import torch
+        dev = _here()
+        q, stride, qs = self._queries(queries, dev)
+        nq, n = q.shape[0], self.nrows
+        bias, _ = _bias_arg(bias, 1, n, dev, False)
+        if out is None:
+            out = torch.empty((nq, n), dtype=dtype or torch.float32, device=dev)
+        _tensor(out, "out", _floats(), 2, dev)
+        if out.shape != (nq, n) or dtype not in (None, out.dtype):
+            raise _bad(f"out must be [{nq}, {n}] and of the dtype asked for")
+        ws, wsb = self._workspace(nq, 0, dev)
+        with _OnTorchStream():
+            check(lib().ndbhip_i8_product_device(self._h, _p(q), _types()[q.dtype], _p(qs), nq, stride, _p(bias), _p(out),
+                                                 _types()[out.dtype], _out_rows(out, "out"), _p(ws), wsb))
+        return out
+
+    def search(self, queries, k, bias=None, mask=None):
+        """The k best rows of each query: (ids int64 [nq, k], scores float32 [nq, k]), higher scores first, equal ones by id; places
+        no row fills hold -1 and -inf.  ndbhip_i8_search_device.  bias: float32 [nrows]; mask: as in adjust_scores.  numpy float32
+        queries (and numpy bias, mask uint32 / int32) take the host form and return numpy arrays."""
+        import torch
+        if isinstance(queries, np.ndarray):
+            return self._search_host(queries, int(k), bias, mask)
+        dev = _here()
+        q, stride, qs = self._queries(queries, dev)
+        nq, n, k = q.shape[0], self.nrows, int(k)
+        bias, _ = _bias_arg(bias, 1, n, dev, False)
+        mask, mstride = _mask_arg(mask, nq, n, dev)
+        ws, wsb = self._workspace(nq, k, dev)
+        ids = torch.empty((nq, max(k, 0)), dtype=torch.int64, device=dev)
+        scores = torch.empty((nq, max(k, 0)), dtype=torch.float32, device=dev)
+        with _OnTorchStream():
+            check(lib().ndbhip_i8_search_device(self._h, _p(q), _types()[q.dtype], _p(qs), nq, stride, _p(bias), _p(mask), mstride, k,
+                                                _p(ids), _p(scores), _p(ws), wsb))
+        return ids, scores
+
+    def _search_host(self, queries, k, bias, mask):
+        q = np.ascontiguousarray(queries, dtype=np.float32)
+        n = self.nrows
+        if q.ndim != 2 or q.shape[1] != self.dim:
+            raise _bad(f"queries must be [nq, {self.dim}]")
+        p = lambda a: None if a is None else a.ctypes.data_as(C.c_void_p)     # noqa: E731
+        if bias is not None:
+            bias = np.ascontiguousarray(bias, dtype=np.float32)
+            if bias.shape != (n,):
+                raise _bad(f"bias must be [{n}]")
+        mstride = 0
+        if mask is not None:
+            mask = np.ascontiguousarray(mask)
+            if mask.dtype not in (np.uint32, np.int32):
+                raise _bad("mask must be uint32 or int32 words")
+            m = mask[None] if mask.ndim == 1 else mask
+            if m.ndim != 2 or m.shape[0] not in (1, q.shape[0]) or m.shape[1] < (n + 31) // 32:
+                raise _bad(f"mask must be [words] or [1 or {q.shape[0]}, words] with at least {(n + 31) // 32} words of 32 rows")
+            mstride = 0 if m.shape[0] == 1 else m.shape[1]
+        ids = np.empty((q.shape[0], max(k, 0)), dtype=np.int64)
+        scores = np.empty((q.shape[0], max(k, 0)), dtype=np.float32)
+        check(lib().ndbhip_i8_search(self._h, p(q), q.shape[0], p(bias), p(mask), mstride, k, p(ids), p(scores)))
+        return ids, scores
