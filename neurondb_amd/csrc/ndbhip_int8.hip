@@ -44,7 +44,12 @@ template <> struct I8Elem<float>
 template <> struct I8Elem<__half>
 {
 	static __device__ __forceinline__ float load(__half v) { return __half2float(v); }
-	static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
+	static __device__ __forceinline__ __half store(float v)
+	{
+		/* (left to itself the compiler folds a product and this into one mixed instruction that skips the rounding to fp32) */
+		asm("" : "+v"(v));
+		return __float2half_rn(v);
+	}
 };
 template <> struct I8Elem<__hip_bfloat16>
 {
@@ -312,7 +317,7 @@ i8_score(int dot, float rs, float qs)
  * The block of sums of row block rb and query block qb: lane l has query l % 32 and, in register 4 g + j, row
  * 8 g + 4 (l / 32) + j.
  */
-template <class T>
+template <bool BIAS, class T>
 __device__ __forceinline__ void
 i8_write_scores(const I8Out &o, uint32_t rb, uint32_t qb, const i8_v16i &acc)
 {
@@ -337,7 +342,7 @@ i8_write_scores(const I8Out &o, uint32_t rb, uint32_t qb, const i8_v16i &acc)
 #pragma unroll
 		for (int j = 0; j < 4; j++)
 		{
-			if (o.bias && r + j < o.n)
+			if (BIAS && r + j < o.n)
 				s[j] = s[j] + o.bias[r + j];
 			v.v[j] = I8Elem<T>::store(s[j]);
 		}
@@ -351,46 +356,92 @@ i8_write_scores(const I8Out &o, uint32_t rb, uint32_t qb, const i8_v16i &acc)
 	}
 }
 
-/* the largest score that takes part among the 32 rows of block rb, for the lane's query (both halves of the wave hold it) */
+/*
+ * The largest score that takes part among the 32 rows of block rb, for the lane's query (both halves of the wave hold it).
+ * rs: the block's 32 row scales; bias: its nbias (1 .. 32) biases, padding rows have none.  fmaxf drops NaN: rows of NaN scores, padding rows among them, never take
+ * part.  A product with a positive finite query scale rises with its other factor and so does its rounding, hence without
+ * a bias RN(t * qs) is taken of the largest t only.
+ */
+template <bool BIAS, bool MASK>
 __device__ __forceinline__ float
-i8_block_max(const I8Out &o, uint32_t rb, uint32_t q, const i8_v16i &acc)
+i8_block_max(const float *rs, const float *bias, uint32_t nbias, uint32_t bits, float qs, const i8_v16i &acc)
 {
-	const int	lane = threadIdx.x & 63;
-	const uint32_t r0 = rb * 32 + 4 * (lane >> 5);
-	const bool	in = q < o.nq && rb * 32 < o.n;
-	const float qs = in ? o.qscale[q] : 0.0f;
-	const uint32_t bits = in && o.mask ? o.mask[(int64_t) q * o.mask_stride + rb] : 0xFFFFFFFFu;
+	const int	h = (threadIdx.x & 63) >> 5;
+	const bool	rises = qs > 0.0f && qs < __builtin_inff();
 	float		m = I8_NINF;
 
-#pragma unroll
-	for (int g4 = 0; g4 < 4; g4++)
+	if (!BIAS && __all(rises))
 	{
-		const uint32_t r = r0 + 8 * g4;
-		const float4 rs = *(const float4 *) (o.rscale + r);
-		const float rv[4] = {rs.x, rs.y, rs.z, rs.w};
+#pragma unroll
+		for (int g4 = 0; g4 < 4; g4++)
+		{
+			const float4 r4 = *(const float4 *) (rs + 8 * g4 + 4 * h);
+			const float rv[4] = {r4.x, r4.y, r4.z, r4.w};
 
 #pragma unroll
-		for (int j = 0; j < 4; j++)
-		{
-			float		s = i8_score(acc[4 * g4 + j], rv[j], qs);
+			for (int j = 0; j < 4; j++)
+			{
+				float		t = (float) acc[4 * g4 + j] * rv[j];
 
-			if (o.bias && r + j < o.n)
-				s = s + o.bias[r + j];
-			/* (a comparison with NaN is false: NaN scores, padding rows among them, never take part) */
-			if ((bits >> ((r + j) & 31) & 1u) && s > m)
-				m = s;
+				if (MASK)
+				{
+					const uint32_t in = (uint32_t) __builtin_amdgcn_sbfe((int) (bits >> (4 * h)), 8 * g4 + j, 1);
+
+					t = __uint_as_float((in & __float_as_uint(t)) | (~in & 0xFF800000u));
+				}
+				m = fmaxf(m, t);
+			}
 		}
+		m = m > I8_NINF ? m * qs : I8_NINF;
 	}
+	else
+#pragma unroll
+		for (int g4 = 0; g4 < 4; g4++)
+		{
+			const float4 r4 = *(const float4 *) (rs + 8 * g4 + 4 * h);
+			const float rv[4] = {r4.x, r4.y, r4.z, r4.w};
+
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+			{
+				float		t = i8_score(acc[4 * g4 + j], rv[j], qs);
+
+				if (BIAS)
+					t = t + bias[min((uint32_t) (8 * g4 + 4 * h + j), nbias - 1)];
+				if (MASK)
+				{
+					const uint32_t in = (uint32_t) __builtin_amdgcn_sbfe((int) (bits >> (4 * h)), 8 * g4 + j, 1);
+
+					t = __uint_as_float((in & __float_as_uint(t)) | (~in & 0xFF800000u));
+				}
+				m = fmaxf(m, t);
+			}
+		}
 	return fmaxf(m, __shfl_xor(m, 32, 64));
 }
 
-/* The simple form: a wave multiplies one block of 32 rows with TB blocks of 32 queries straight from memory. */
-template <int TB, int MODE, class T>
+__device__ __forceinline__ uint32_t
+i8_mask_word(const I8Out &o, uint32_t rb, uint32_t q)
+{
+	return q < o.nq && rb * 32 < o.n ? o.mask[(int64_t) q * o.mask_stride + rb] : 0u;
+}
+
+/* what an instance of the product kernels does with its sums */
+template <int MODE_, bool BIAS_, bool MASK_, class T_> struct I8Kind
+{
+	static constexpr int MODE = MODE_;		/* 0 writes scores, 1 leaves maxima */
+	static constexpr bool BIAS = BIAS_, MASK = MASK_;
+	typedef T_	T;
+};
+
+/* Few queries: a wave multiplies one block of 32 rows with TB blocks of 32 queries straight from memory. */
+template <int TB, class KIND>
 __global__ __launch_bounds__(256) void
 k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrb, uint32_t nqb, I8Out o)
 {
 	const int	lane = threadIdx.x & 63;
-	const uint32_t rb = blockIdx.x * 4 + (threadIdx.x >> 6);
+	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const uint32_t rb = blockIdx.x * 4 + wave;
 	const uint32_t qb0 = blockIdx.y * TB;
 
 	if (rb >= nrb)
@@ -418,17 +469,195 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 	for (int t = 0; t < TB; t++)
 		if (qb0 + t < nqb)
 		{
-			if (MODE == 0)
-				i8_write_scores<T>(o, rb, qb0 + t, acc[t]);
+			if (KIND::MODE == 0)
+				i8_write_scores<KIND::BIAS, typename KIND::T>(o, rb, qb0 + t, acc[t]);
 			else
 			{
 				const uint32_t q = (qb0 + t) * 32 + (lane & 31);
-				const float m = i8_block_max(o, rb, q, acc[t]);
+				const float m = i8_block_max<KIND::BIAS, KIND::MASK>(o.rscale + rb * 32, o.bias + rb * 32, min(32u, o.n - rb * 32),
+																	 KIND::MASK ? i8_mask_word(o, rb, q) : 0u,
+																	 q < o.nq ? o.qscale[q] : 1.0f, acc[t]);
 
 				if (lane < 32 && q < o.nq)
 					o.gmax[(size_t) q * o.ngp + rb] = m;
 			}
 		}
+}
+
+/* ------------------------------------------------------------------ */
+
+/* every request of this wave older than the newest N has landed */
+template <int N>
+__device__ __forceinline__ void
+i8_wait_vm()
+{
+	static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
+	asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+
+/* lane i copies the 16 bytes at base + voff to LDS at la + 16 i (voff: 16 i and whatever is the same in all lanes).  Inline
+ * asm: the compiler would put a wait for ALL such copies in front of every LDS read of a ring it cannot tell apart, and
+ * M0, which only these copies use here, is written right before each. */
+__device__ __forceinline__ void
+i8_dma16(const unsigned char *base, uint32_t voff, uint32_t la)
+{
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(la), "v"(voff), "s"(base) : "memory");
+}
+
+__device__ __forceinline__ const unsigned char *
+i8_uniform(const unsigned char *p)
+{
+	const uint64_t v = (uint64_t) p;
+	const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t) v), hi = __builtin_amdgcn_readfirstlane((uint32_t) (v >> 32));
+
+	return (const unsigned char *) (((uint64_t) hi << 32) | lo);
+}
+
+/*
+ * Many queries: a block multiplies a tile of NWR * WR row blocks with one of NWQ * WQ query blocks, wave (wr, wq) of it
+ * WR x WQ blocks of 32 x 32 sums in registers.  Both operands pass through LDS in stages of 64 dimensions (2 KiB a block
+ * of rows or queries, copied as they lie in memory), a ring of NBUF stages that the copies run NBUF - 1 ahead of.
+ * The operand layout makes every LDS read one conflict-free 16 bytes a lane.
+ */
+template <int WR_, int WQ_, int NWR_, int NWQ_, int NBUF_> struct I8Tile
+{
+	static constexpr int WR = WR_, WQ = WQ_, NWR = NWR_, NWQ = NWQ_, NBUF = NBUF_;
+	static constexpr int NW = NWR * NWQ;
+	static constexpr int RB = WR * NWR, QB = WQ * NWQ;		/* blocks of the tile */
+	static constexpr int STAGE = (RB + QB) * 2048;
+	static constexpr int PER = 2 * (RB + QB) / NW;			/* copies of 1 KiB a wave makes per stage */
+	static_assert(2 * (RB + QB) % NW == 0, "every wave copies the same number of KiB");
+	static_assert((NBUF - 1) * PER < 64, "vmcnt is a 6-bit counter");
+};
+
+template <class TILE, class KIND>
+__global__ __launch_bounds__(64 * TILE::NW, 1) void
+k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrt, uint32_t nqt, I8Out o)
+{
+	constexpr int WR = TILE::WR, WQ = TILE::WQ, RB = TILE::RB, QB = TILE::QB, NBUF = TILE::NBUF, PER = TILE::PER;
+	__shared__ __attribute__((aligned(1024))) unsigned char ring[NBUF * TILE::STAGE];
+	__shared__ __attribute__((aligned(16))) float s_rs[RB * 32], s_bias[KIND::BIAS ? RB * 32 : 4];
+	const int	lane = threadIdx.x & 63;
+	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int	wq = wave % TILE::NWQ, wr = wave / TILE::NWQ;
+	/*
+	 * Blocks go round the 8 XCDs; the ones an XCD runs together take all query tiles of one row tile, then of the next,
+	 * so that its L2 holds the queries and sees each row tile once.
+	 */
+	const uint32_t j = blockIdx.x >> 3;
+	const uint32_t qt = j % nqt, rt = (j / nqt) * 8 + (blockIdx.x & 7);
+
+	if (rt >= nrt)
+		return;
+	const uint32_t rb0 = rt * RB, qb0 = qt * QB;
+	const uint32_t blk = kp * 32;			/* bytes of a block */
+	const unsigned char *rbase = i8_uniform(rows + (size_t) rb0 * blk);
+	const unsigned char *qbase = i8_uniform(queries + (size_t) qb0 * blk);
+	const uint32_t ring_la = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) ring;
+	const uint32_t ns = kp / 64;
+
+	for (int i = threadIdx.x; i < RB * 32; i += 64 * TILE::NW)
+	{
+		const uint32_t r = rb0 * 32 + i;
+
+		s_rs[i] = o.rscale[r];
+		if (KIND::BIAS)
+			s_bias[i] = r < o.n ? o.bias[r] : 0.0f;
+	}
+
+	auto		request = [&](uint32_t s) {
+		const uint32_t la = ring_la + (s % NBUF) * TILE::STAGE;
+
+#pragma unroll
+		for (int i = 0; i < PER; i++)
+		{
+			const int	c = wave * PER + i;			/* KiB c of the stage: block c / 2, half c % 2 */
+			const bool	isq = c >= 2 * RB;
+			const uint32_t off = (uint32_t) ((isq ? c - 2 * RB : c) >> 1) * blk + s * 2048u + (c & 1) * 1024u;
+
+			i8_dma16(isq ? qbase : rbase, off + lane * 16, la + c * 1024);
+		}
+	};
+	i8_v16i		acc[WR][WQ];
+
+#pragma unroll
+	for (int i = 0; i < WR; i++)
+#pragma unroll
+		for (int t = 0; t < WQ; t++)
+#pragma unroll
+			for (int e = 0; e < 16; e++)
+				acc[i][t][e] = 0;
+#pragma unroll
+	for (int s = 0; s < NBUF - 1; s++)
+		if ((uint32_t) s < ns)
+			request(s);
+	for (uint32_t s = 0; s < ns; s++)
+	{
+		/* stage s has landed (the stages behind it may still be on their way; near the end there are fewer of them) ... */
+		if (s + NBUF - 1 <= ns)
+			i8_wait_vm<(NBUF - 2) * PER>();
+		else
+			i8_wait_vm<0>();
+		/* ... for every wave, and every wave has read what it needs of the stage before, whose place is filled again */
+		asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+		if (s + NBUF - 1 < ns)
+			request(s + NBUF - 1);
+		const unsigned char *st = ring + (s % NBUF) * TILE::STAGE + lane * 16;
+
+#pragma unroll
+		for (int h = 0; h < 2; h++)
+		{
+			i8_v4i		av[WR], bv[WQ];
+
+#pragma unroll
+			for (int i = 0; i < WR; i++)
+				av[i] = *(const i8_v4i *) (st + (wr * WR + i) * 2048 + h * 1024);
+#pragma unroll
+			for (int t = 0; t < WQ; t++)
+				bv[t] = *(const i8_v4i *) (st + (RB + wq * WQ + t) * 2048 + h * 1024);
+#pragma unroll
+			for (int i = 0; i < WR; i++)
+#pragma unroll
+				for (int t = 0; t < WQ; t++)
+					acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], bv[t], acc[i][t], 0, 0, 0);
+		}
+	}
+	if (KIND::MODE == 0)
+	{
+#pragma unroll
+		for (int t = 0; t < WQ; t++)
+#pragma unroll
+			for (int i = 0; i < WR; i++)
+				i8_write_scores<KIND::BIAS, typename KIND::T>(o, rb0 + wr * WR + i, qb0 + wq * WQ + t, acc[i][t]);
+	}
+	else
+	{
+#pragma unroll
+		for (int t = 0; t < WQ; t++)
+		{
+			const uint32_t q = (qb0 + wq * WQ + t) * 32 + (lane & 31);
+			const float qs = q < o.nq ? o.qscale[q] : 1.0f;		/* (a padding query's NaN would cost its neighbours the short way) */
+			float		m[WR];
+
+#pragma unroll
+			for (int i = 0; i < WR; i++)
+				m[i] = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs + (wr * WR + i) * 32, s_bias + (KIND::BIAS ? (wr * WR + i) * 32 : 0), 32u,
+															KIND::MASK ? i8_mask_word(o, rb0 + wr * WR + i, q) : 0u, qs, acc[i][t]);
+			if (q < o.nq && lane < 32)
+			{
+				float	   *gm = o.gmax + (size_t) q * o.ngp + rb0 + wr * WR;
+
+				if constexpr (WR == 4)
+					*(float4 *) gm = make_float4(m[0], m[1], m[2], m[3]);
+				else if constexpr (WR == 2)
+					*(float2 *) gm = make_float2(m[0], m[1]);
+				else
+#pragma unroll
+					for (int i = 0; i < WR; i++)
+						gm[i] = m[i];
+			}
+		}
+	}
 }
 
 /* ================================================================== */
@@ -1098,16 +1327,43 @@ i8_take_queries(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_
 	return i8_quantize_any<true>(q, q_type, m, w.nqp, t->dim, q_stride, codes, 0, t->kp, scales);
 }
 
-template <int MODE, class T>
+typedef I8Tile<4, 2, 2, 4, 3> I8Tile256;
+
+template <class KIND>
 static int
-i8_multiply(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
+i8_multiply_kind(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
 {
 	const uint32_t nrb = (o.n + 31) / 32, nqb = (o.nq + 31) / 32;
 
-	hipLaunchKernelGGL((k_i8_stream<2, MODE, T>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
-					   nrb, nqb, o);
+	if (o.nq > 64)
+	{
+		const uint32_t nrt = (nrb + I8Tile256::RB - 1) / I8Tile256::RB, nqt = (nqb + I8Tile256::QB - 1) / I8Tile256::QB;
+
+		hipLaunchKernelGGL((k_i8_tile<I8Tile256, KIND>), dim3((nrt + 7) / 8 * 8 * nqt), dim3(64 * I8Tile256::NW), 0, g.stream, t->d_codes,
+						   queries, t->kp, nrt, nqt, o);
+	}
+	else
+		hipLaunchKernelGGL((k_i8_stream<2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
+						   nrb, nqb, o);
 	HIP_TRY(hipGetLastError());
 	return NDBHIP_OK;
+}
+
+template <class T>
+static int
+i8_multiply_scores(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
+{
+	return o.bias ? i8_multiply_kind<I8Kind<0, true, false, T>>(t, queries, o) : i8_multiply_kind<I8Kind<0, false, false, T>>(t, queries, o);
+}
+
+static int
+i8_multiply_maxima(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
+{
+	if (o.mask)
+		return o.bias ? i8_multiply_kind<I8Kind<1, true, true, float>>(t, queries, o) :
+			i8_multiply_kind<I8Kind<1, false, true, float>>(t, queries, o);
+	return o.bias ? i8_multiply_kind<I8Kind<1, true, false, float>>(t, queries, o) :
+		i8_multiply_kind<I8Kind<1, false, false, float>>(t, queries, o);
 }
 
 extern "C" int
@@ -1150,8 +1406,8 @@ ndbhip_i8_product_device(const ndbhip_i8 *t, const void *d_q, int q_type, const 
 		o.nq = (uint32_t) m;
 		const unsigned char *qc = (const unsigned char *) d_ws + w.q_off;
 
-		rc = out_type == NDBHIP_F32 ? i8_multiply<0, float>(t, qc, o) : out_type == NDBHIP_F16 ? i8_multiply<0, __half>(t, qc, o) :
-			i8_multiply<0, __hip_bfloat16>(t, qc, o);
+		rc = out_type == NDBHIP_F32 ? i8_multiply_scores<float>(t, qc, o) : out_type == NDBHIP_F16 ? i8_multiply_scores<__half>(t, qc, o) :
+			i8_multiply_scores<__hip_bfloat16>(t, qc, o);
 		if (rc)
 			return rc;
 	}
@@ -1212,7 +1468,7 @@ ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const f
 		o.ngp = w.ngp;
 		o.n = (uint32_t) t->n;
 		o.nq = (uint32_t) m;
-		if ((rc = i8_multiply<1, float>(t, qc, o)))
+		if ((rc = i8_multiply_maxima(t, qc, o)))
 			return rc;
 		hipLaunchKernelGGL(k_i8_pick, dim3(m), dim3(256), 0, g.stream, o.gmax, w.ngp, w.ng, (uint32_t) k, picked, npicked);
 		hipLaunchKernelGGL(k_i8_rescore, dim3((k + 3) / 4, m), dim3(256), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, picked,
