@@ -314,36 +314,35 @@ i8_score(int dot, float rs, float qs)
 }
 
 /*
- * The block of sums of row block rb and query block qb: lane l has query l % 32 and, in register 4 g + j, row
- * 8 g + 4 (l / 32) + j.
+ * The block of sums of a row block rb and a query block: lane l has query l % 32 of it and, in register 4 g + j, row
+ * 8 g + 4 (l / 32) + j.  rs, bias: from the row block's first on, in memory or in LDS; rows behind the last have a scale but no bias.
  */
 template <bool BIAS, class T>
 __device__ __forceinline__ void
-i8_write_scores(const I8Out &o, uint32_t rb, uint32_t qb, const i8_v16i &acc)
+i8_write_scores(const I8Out &o, const float *rs, const float *bias, uint32_t rb, uint32_t q, float qs, const i8_v16i &acc)
 {
-	const int	lane = threadIdx.x & 63;
-	const uint32_t q = qb * 32 + (lane & 31);
-	const uint32_t r0 = rb * 32 + 4 * (lane >> 5);
+	const int	h = (threadIdx.x & 63) >> 5;
+	const uint32_t r0 = rb * 32 + 4 * h;
 
-	if (q >= o.nq)
+	if (q >= o.nq || rb * 32 >= o.n)
 		return;
-	const float qs = o.qscale[q];
+	const uint32_t left = o.n - rb * 32;
 	T		   *out = (T *) o.out + (int64_t) q * o.ostride;
 
 #pragma unroll
 	for (int g4 = 0; g4 < 4; g4++)
 	{
 		const uint32_t r = r0 + 8 * g4;
-		const float4 rs = *(const float4 *) (o.rscale + r);
-		float		s[4] = {i8_score(acc[4 * g4], rs.x, qs), i8_score(acc[4 * g4 + 1], rs.y, qs),
-			i8_score(acc[4 * g4 + 2], rs.z, qs), i8_score(acc[4 * g4 + 3], rs.w, qs)};
+		const float4 r4 = *(const float4 *) (rs + 8 * g4 + 4 * h);
+		float		s[4] = {i8_score(acc[4 * g4], r4.x, qs), i8_score(acc[4 * g4 + 1], r4.y, qs),
+			i8_score(acc[4 * g4 + 2], r4.z, qs), i8_score(acc[4 * g4 + 3], r4.w, qs)};
 		I8Vec<T, 4> v;
 
 #pragma unroll
 		for (int j = 0; j < 4; j++)
 		{
-			if (BIAS && r + j < o.n)
-				s[j] = s[j] + o.bias[r + j];
+			if (BIAS)
+				s[j] = s[j] + bias[min((uint32_t) (8 * g4 + 4 * h + j), left - 1)];
 			v.v[j] = I8Elem<T>::store(s[j]);
 		}
 		if (o.ovec && r + 4 <= o.n)
@@ -469,11 +468,12 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 	for (int t = 0; t < TB; t++)
 		if (qb0 + t < nqb)
 		{
+			const uint32_t q = (qb0 + t) * 32 + (lane & 31);
+
 			if (KIND::MODE == 0)
-				i8_write_scores<KIND::BIAS, typename KIND::T>(o, rb, qb0 + t, acc[t]);
+				i8_write_scores<KIND::BIAS, typename KIND::T>(o, o.rscale + rb * 32, o.bias + rb * 32, rb, q, o.qscale[q], acc[t]);
 			else
 			{
-				const uint32_t q = (qb0 + t) * 32 + (lane & 31);
 				const float m = i8_block_max<KIND::BIAS, KIND::MASK>(o.rscale + rb * 32, o.bias + rb * 32, min(32u, o.n - rb * 32),
 																	 KIND::MASK ? i8_mask_word(o, rb, q) : 0u,
 																	 q < o.nq ? o.qscale[q] : 1.0f, acc[t]);
@@ -495,169 +495,246 @@ i8_wait_vm()
 	asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
 }
 
-/* lane i copies the 16 bytes at base + voff to LDS at la + 16 i (voff: 16 i and whatever is the same in all lanes).  Inline
- * asm: the compiler would put a wait for ALL such copies in front of every LDS read of a ring it cannot tell apart, and
- * M0, which only these copies use here, is written right before each. */
+/* lane i copies 16 (4) bytes at base + voff to LDS at la + 16 (4) i.  Inline asm: the compiler would put a wait for ALL
+ * such copies in front of every LDS read of a ring it cannot tell apart, and M0, which only these copies use here, is
+ * written right before each (the wait states cover M0 and a base that a vector instruction has just put into its scalar
+ * registers).  Not a memory clobber: the barriers around the ring are, and copies may move between reads. */
 __device__ __forceinline__ void
-i8_dma16(const unsigned char *base, uint32_t voff, uint32_t la)
+i8_dma16(const void *base, uint32_t voff, uint32_t la)
 {
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(la), "v"(voff), "s"(base) : "memory");
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(la), "v"(voff), "s"(base));
+}
+__device__ __forceinline__ void
+i8_dma4(const void *base, uint32_t voff, uint32_t la)
+{
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" :: "s"(la), "v"(voff), "s"(base));
 }
 
-__device__ __forceinline__ const unsigned char *
-i8_uniform(const unsigned char *p)
+template <class T>
+__device__ __forceinline__ T *
+i8_uniform(T *p)
 {
 	const uint64_t v = (uint64_t) p;
 	const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t) v), hi = __builtin_amdgcn_readfirstlane((uint32_t) (v >> 32));
 
-	return (const unsigned char *) (((uint64_t) hi << 32) | lo);
+	return (T *) (((uint64_t) hi << 32) | lo);
+}
+
+__device__ __forceinline__ uint32_t
+i8_lds(const void *p)
+{
+	return (uint32_t) (uintptr_t) (__attribute__((address_space(3))) const unsigned char *) p;
 }
 
 /*
- * Many queries: a block multiplies a tile of NWR * WR row blocks with one of NWQ * WQ query blocks, wave (wr, wq) of it
- * WR x WQ blocks of 32 x 32 sums in registers.  Both operands pass through LDS in stages of 64 dimensions (2 KiB a block
- * of rows or queries, copied as they lie in memory), a ring of NBUF stages that the copies run NBUF - 1 ahead of.
- * The operand layout makes every LDS read one conflict-free 16 bytes a lane.
+ * Many queries: a block of 2 x NWQ waves multiplies tiles of 256 rows x 64 NWQ queries, wave (wr, wq) of it 128 x 64 sums
+ * in registers.  Both operands pass through LDS in stages of 64 dimensions (2 KiB a block of 32 rows
+ * or queries, copied as they lie in memory; an LDS read is 16 bytes a lane without conflicts), a ring of NBUF.
+ *
+ * Two waves a SIMD do not hide each other's waits (they meet at the same barriers), so the stream is pipelined by hand.  A
+ * stage is two halves of 32 dimensions
+ * (one matrix instruction deep): while one half is multiplied, the operands of the next are read, also across the
+ * barrier that opens the next stage.  Tiles follow each other without a gap: the ring runs into the next tile of the
+ * block, whose first operands are in registers when the sums of this one are written out.
+ *
+ * Row scales, query scales and biases of a tile come through LDS the same way, with the copies of its first stage: a load
+ * of the wave's own would have to wait for every copy requested before it (requests retire in order).
  */
-template <int WR_, int WQ_, int NWR_, int NWQ_, int NBUF_> struct I8Tile
+#define I8_TR 8					/* blocks of rows in a tile */
+#define I8_NBUF 3
+#define I8_SLOTS 4				/* tiles whose scales are in LDS: the ring is at most NBUF tiles ahead */
+
+#define I8_WQ 2					/* blocks of queries a wave multiplies */
+
+template <int NWQ> struct I8Tile
 {
-	static constexpr int WR = WR_, WQ = WQ_, NWR = NWR_, NWQ = NWQ_, NBUF = NBUF_;
-	static constexpr int NW = NWR * NWQ;
-	static constexpr int RB = WR * NWR, QB = WQ * NWQ;		/* blocks of the tile */
-	static constexpr int STAGE = (RB + QB) * 2048;
-	static constexpr int PER = 2 * (RB + QB) / NW;			/* copies of 1 KiB a wave makes per stage */
-	static_assert(2 * (RB + QB) % NW == 0, "every wave copies the same number of KiB");
-	static_assert((NBUF - 1) * PER < 64, "vmcnt is a 6-bit counter");
+	static constexpr int NW = 2 * NWQ;
+	static constexpr int QB = NWQ * I8_WQ;					/* blocks of queries in a tile */
+	static constexpr int STAGE = (I8_TR + QB) * 2048;
+	static constexpr int PER = 2 * (I8_TR + QB) / NW;		/* copies of 1 KiB a wave makes per stage */
 };
 
-template <class TILE, class KIND>
-__global__ __launch_bounds__(64 * TILE::NW, 1) void
+template <int NWQ, class KIND>
+__global__ __launch_bounds__(128 * NWQ, 2) void
 k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrt, uint32_t nqt, I8Out o)
 {
-	constexpr int WR = TILE::WR, WQ = TILE::WQ, RB = TILE::RB, QB = TILE::QB, NBUF = TILE::NBUF, PER = TILE::PER;
-	__shared__ __attribute__((aligned(1024))) unsigned char ring[NBUF * TILE::STAGE];
-	__shared__ __attribute__((aligned(16))) float s_rs[RB * 32], s_bias[KIND::BIAS ? RB * 32 : 4];
+	typedef I8Tile<NWQ> TILE;
+	constexpr int QB = TILE::QB, PER = TILE::PER, WQ = I8_WQ;
+	__shared__ __attribute__((aligned(1024))) unsigned char ring[I8_NBUF * TILE::STAGE];
+	__shared__ __attribute__((aligned(1024))) float s_rs[I8_SLOTS][256];
+	__shared__ __attribute__((aligned(1024))) float s_qs[I8_SLOTS][256];
+	__shared__ __attribute__((aligned(1024))) float s_bias[KIND::BIAS ? I8_SLOTS : 1][256];
 	const int	lane = threadIdx.x & 63;
 	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const int	wq = wave % TILE::NWQ, wr = wave / TILE::NWQ;
+	const int	wq = wave % NWQ, wr = wave / NWQ;
 	/*
-	 * Blocks go round the 8 XCDs; the ones an XCD runs together take all query tiles of one row tile, then of the next,
-	 * so that its L2 holds the queries and sees each row tile once.
+	 * Blocks go round the 8 XCDs.  An XCD takes every eighth row tile and of each all query tiles one after the other, dealt
+	 * to its blocks in turn: its L2 holds the queries and sees each row tile once.
 	 */
-	const uint32_t j = blockIdx.x >> 3;
-	const uint32_t qt = j % nqt, rt = (j / nqt) * 8 + (blockIdx.x & 7);
-
-	if (rt >= nrt)
-		return;
-	const uint32_t rb0 = rt * RB, qb0 = qt * QB;
+	const uint32_t xcd = blockIdx.x & 7, nslot = gridDim.x >> 3;
+	const uint32_t mine = nrt > xcd ? (nrt - xcd + 7) / 8 * nqt : 0;
 	const uint32_t blk = kp * 32;			/* bytes of a block */
-	const unsigned char *rbase = i8_uniform(rows + (size_t) rb0 * blk);
-	const unsigned char *qbase = i8_uniform(queries + (size_t) qb0 * blk);
-	const uint32_t ring_la = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) ring;
 	const uint32_t ns = kp / 64;
+	const uint32_t ring_la = i8_lds(ring);
+	const uint32_t first = blockIdx.x >> 3;
 
-	for (int i = threadIdx.x; i < RB * 32; i += 64 * TILE::NW)
-	{
-		const uint32_t r = rb0 * 32 + i;
-
-		s_rs[i] = o.rscale[r];
-		if (KIND::BIAS)
-			s_bias[i] = r < o.n ? o.bias[r] : 0.0f;
-	}
-
-	auto		request = [&](uint32_t s) {
-		const uint32_t la = ring_la + (s % NBUF) * TILE::STAGE;
-
-#pragma unroll
-		for (int i = 0; i < PER; i++)
+	if (first >= mine)
+		return;
+	const uint32_t dr = nslot / nqt, dq = nslot % nqt;		/* from a tile of this block to its next */
+	auto		forward = [&](uint32_t &rt, uint32_t &qt) {
+		rt += 8 * dr;
+		qt += dq;
+		if (qt >= nqt)
 		{
-			const int	c = wave * PER + i;			/* KiB c of the stage: block c / 2, half c % 2 */
-			const bool	isq = c >= 2 * RB;
-			const uint32_t off = (uint32_t) ((isq ? c - 2 * RB : c) >> 1) * blk + s * 2048u + (c & 1) * 1024u;
-
-			i8_dma16(isq ? qbase : rbase, off + lane * 16, la + c * 1024);
+			qt -= nqt;
+			rt += 8;
 		}
 	};
-	i8_v16i		acc[WR][WQ];
 
-#pragma unroll
-	for (int i = 0; i < WR; i++)
+	/* the copies' place in the stream of stages; behind the last tile they go over that one again, read by nobody */
+	uint32_t	c_rt = first / nqt * 8 + xcd, c_qt = first % nqt, c_left = (mine - first + nslot - 1) / nslot, c_s = 0, c_slot = 0, c_buf = 0;
+	const unsigned char *c_r = i8_uniform(rows + (size_t) c_rt * I8_TR * blk), *c_q = i8_uniform(queries + (size_t) c_qt * QB * blk);
+
+	/* the first copies of a tile: its scales (and biases, the rows behind the last take the last one's) */
+	auto		c_scales = [&]() {
+		if (wave == 0)
+			i8_dma16(i8_uniform(o.rscale + (size_t) c_rt * 256), lane * 16, i8_lds(s_rs) + c_slot * 1024);
+		if (wave == 1)
+			i8_dma16(i8_uniform(o.qscale + (size_t) c_qt * QB * 32), (lane & (QB * 8 - 1)) * 16, i8_lds(s_qs) + c_slot * 1024);
+		if (KIND::BIAS && wave < 4)
+			i8_dma4(i8_uniform(o.bias + (size_t) c_rt * 256), min(wave * 64u + lane, o.n - 1 - c_rt * 256) * 4,
+					i8_lds(s_bias) + c_slot * 1024 + wave * 256);
+	};
+	auto		c_copy = [&](int i) {
+		const int	c = wave * PER + i;			/* KiB c of the stage: block c / 2, half c % 2 */
+		const bool	isq = c >= 2 * I8_TR;
+		const uint32_t off = (uint32_t) ((isq ? c - 2 * I8_TR : c) >> 1) * blk + c_s * 2048u + (c & 1) * 1024u;
+
+		i8_dma16(isq ? c_q : c_r, off + lane * 16, ring_la + c_buf * TILE::STAGE + c * 1024);
+	};
+	auto		c_next = [&]() {
+		c_buf = c_buf + 1 == I8_NBUF ? 0 : c_buf + 1;
+		if (++c_s == ns)
+		{
+			c_s = 0;
+			c_slot = (c_slot + 1) & (I8_SLOTS - 1);
+			if (--c_left > 0)
+			{
+				forward(c_rt, c_qt);
+				c_r = i8_uniform(rows + (size_t) c_rt * I8_TR * blk);
+				c_q = i8_uniform(queries + (size_t) c_qt * QB * blk);
+			}
+			else
+				c_left = 1;
+		}
+	};
+
+	i8_v4i		av[2][4], bv[2][WQ];
+	i8_v16i		acc[4][WQ];
+	const unsigned char *lane_ring = ring + lane * 16;
+	auto		read = [&](uint32_t buf, int h) {
+		const unsigned char *st = lane_ring + buf * TILE::STAGE + h * 1024;
+
 #pragma unroll
 		for (int t = 0; t < WQ; t++)
+			bv[h][t] = *(const i8_v4i *) (st + (I8_TR + wq * WQ + t) * 2048);
 #pragma unroll
-			for (int e = 0; e < 16; e++)
-				acc[i][t][e] = 0;
+		for (int i = 0; i < 4; i++)
+			av[h][i] = *(const i8_v4i *) (st + (wr * 4 + i) * 2048);
+	};
+
 #pragma unroll
-	for (int s = 0; s < NBUF - 1; s++)
-		if ((uint32_t) s < ns)
-			request(s);
-	for (uint32_t s = 0; s < ns; s++)
+	for (int s = 0; s < I8_NBUF; s++)
 	{
-		/* stage s has landed (the stages behind it may still be on their way; near the end there are fewer of them) ... */
-		if (s + NBUF - 1 <= ns)
-			i8_wait_vm<(NBUF - 2) * PER>();
-		else
-			i8_wait_vm<0>();
-		/* ... for every wave, and every wave has read what it needs of the stage before, whose place is filled again */
-		asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-		if (s + NBUF - 1 < ns)
-			request(s + NBUF - 1);
-		const unsigned char *st = ring + (s % NBUF) * TILE::STAGE + lane * 16;
-
+		if (c_s == 0)
+			c_scales();
 #pragma unroll
-		for (int h = 0; h < 2; h++)
-		{
-			i8_v4i		av[WR], bv[WQ];
+		for (int i = 0; i < PER; i++)
+			c_copy(i);
+		c_next();
+	}
+	i8_wait_vm<(I8_NBUF - 1) * PER>();
+	asm volatile("s_barrier" ::: "memory");
+	read(0, 0);
 
+	uint32_t	buf = 0, slot = 0;
+
+	/*
+	 * A stage, its first half's operands in registers.  FIRST: the tile's first stage, sums start from zero.  The next stage
+	 * must have landed for every wave, and every wave must have read the last of this one, before the barrier in the middle;
+	 * behind it this stage's place is filled again.
+	 */
+	auto		stage = [&](auto first_stage) {
+		constexpr bool FIRST = decltype(first_stage)::value;
+		const i8_v16i zero = {};
+
+		read(buf, 1);
+		__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-			for (int i = 0; i < WR; i++)
-				av[i] = *(const i8_v4i *) (st + (wr * WR + i) * 2048 + h * 1024);
+		for (int i = 0; i < 4; i++)
 #pragma unroll
 			for (int t = 0; t < WQ; t++)
-				bv[t] = *(const i8_v4i *) (st + (RB + wq * WQ + t) * 2048 + h * 1024);
+				acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[0][i], bv[0][t], FIRST ? zero : acc[i][t], 0, 0, 0);
+		__builtin_amdgcn_sched_barrier(0);
+		i8_wait_vm<(I8_NBUF - 2) * PER>();
+		asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+		buf = buf + 1 == I8_NBUF ? 0 : buf + 1;
+		read(buf, 0);
+		if (c_s == 0)
+			c_scales();
+		__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-			for (int i = 0; i < WR; i++)
+		for (int i = 0; i < 4; i++)
 #pragma unroll
-				for (int t = 0; t < WQ; t++)
-					acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], bv[t], acc[i][t], 0, 0, 0);
-		}
-	}
-	if (KIND::MODE == 0)
+			for (int t = 0; t < WQ; t++)
+			{
+				acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[1][i], bv[1][t], acc[i][t], 0, 0, 0);
+				if (i * WQ + t < PER)
+					c_copy(i * WQ + t);
+				__builtin_amdgcn_sched_barrier(0);
+			}
+		c_next();
+	};
+	uint32_t	rt = first / nqt * 8 + xcd, qt = first % nqt;
+
+	for (uint32_t left = (mine - first + nslot - 1) / nslot; left > 0; left--)
 	{
-#pragma unroll
-		for (int t = 0; t < WQ; t++)
-#pragma unroll
-			for (int i = 0; i < WR; i++)
-				i8_write_scores<KIND::BIAS, typename KIND::T>(o, rb0 + wr * WR + i, qb0 + wq * WQ + t, acc[i][t]);
-	}
-	else
-	{
+		const uint32_t rb0 = rt * I8_TR + wr * 4, qb0 = qt * QB + wq * WQ;
+
+		stage(std::true_type{});
+		for (uint32_t s = 1; s < ns; s++)
+			stage(std::false_type{});
 #pragma unroll
 		for (int t = 0; t < WQ; t++)
 		{
-			const uint32_t q = (qb0 + wq * WQ + t) * 32 + (lane & 31);
-			const float qs = q < o.nq ? o.qscale[q] : 1.0f;		/* (a padding query's NaN would cost its neighbours the short way) */
-			float		m[WR];
+			const uint32_t q = (qb0 + t) * 32 + (lane & 31);
+			const float qs = s_qs[slot][(wq * WQ + t) * 32 + (lane & 31)];
 
-#pragma unroll
-			for (int i = 0; i < WR; i++)
-				m[i] = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs + (wr * WR + i) * 32, s_bias + (KIND::BIAS ? (wr * WR + i) * 32 : 0), 32u,
-															KIND::MASK ? i8_mask_word(o, rb0 + wr * WR + i, q) : 0u, qs, acc[i][t]);
-			if (q < o.nq && lane < 32)
+			if (KIND::MODE == 0)
 			{
-				float	   *gm = o.gmax + (size_t) q * o.ngp + rb0 + wr * WR;
-
-				if constexpr (WR == 4)
-					*(float4 *) gm = make_float4(m[0], m[1], m[2], m[3]);
-				else if constexpr (WR == 2)
-					*(float2 *) gm = make_float2(m[0], m[1]);
-				else
 #pragma unroll
-					for (int i = 0; i < WR; i++)
-						gm[i] = m[i];
+				for (int i = 0; i < 4; i++)
+					i8_write_scores<KIND::BIAS, typename KIND::T>(o, s_rs[slot] + (wr * 4 + i) * 32,
+																  s_bias[KIND::BIAS ? slot : 0] + (wr * 4 + i) * 32, rb0 + i, q, qs, acc[i][t]);
+			}
+			else
+			{
+				float		m[4];
+
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					m[i] = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs[slot] + (wr * 4 + i) * 32,
+																s_bias[KIND::BIAS ? slot : 0] + (wr * 4 + i) * 32, 32u,
+																KIND::MASK ? i8_mask_word(o, rb0 + i, q) : 0u,
+																q < o.nq ? qs : 1.0f, acc[i][t]);
+				if (q < o.nq && lane < 32)
+					*(float4 *) (o.gmax + (size_t) q * o.ngp + rb0) = make_float4(m[0], m[1], m[2], m[3]);
 			}
 		}
+		slot = (slot + 1) & (I8_SLOTS - 1);
+		forward(rt, qt);
 	}
+	i8_wait_vm<0>();			/* (no copy may be on its way into LDS that is no longer this block's) */
 }
 
 /* ================================================================== */
@@ -1327,7 +1404,17 @@ i8_take_queries(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_
 	return i8_quantize_any<true>(q, q_type, m, w.nqp, t->dim, q_stride, codes, 0, t->kp, scales);
 }
 
-typedef I8Tile<4, 2, 2, 4, 3> I8Tile256;
+template <int NWQ, class KIND>
+static void
+i8_tile_launch(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
+{
+	typedef I8Tile<NWQ> TILE;
+	const uint32_t nrt = (o.n + 255) / 256, nqt = (o.nq + 32 * TILE::QB - 1) / (32 * TILE::QB);
+	/* eight waves a compute unit, its blocks in whole rounds of the XCDs, and no more blocks than have a tile */
+	const uint32_t blocks = std::min(((uint32_t) g.num_cus & ~7u) * (8 / TILE::NW), (nrt + 7) / 8 * 8 * nqt);
+
+	hipLaunchKernelGGL((k_i8_tile<NWQ, KIND>), dim3(blocks), dim3(64 * TILE::NW), 0, g.stream, t->d_codes, queries, t->kp, nrt, nqt, o);
+}
 
 template <class KIND>
 static int
@@ -1335,13 +1422,10 @@ i8_multiply_kind(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &
 {
 	const uint32_t nrb = (o.n + 31) / 32, nqb = (o.nq + 31) / 32;
 
-	if (o.nq > 64)
-	{
-		const uint32_t nrt = (nrb + I8Tile256::RB - 1) / I8Tile256::RB, nqt = (nqb + I8Tile256::QB - 1) / I8Tile256::QB;
-
-		hipLaunchKernelGGL((k_i8_tile<I8Tile256, KIND>), dim3((nrt + 7) / 8 * 8 * nqt), dim3(64 * I8Tile256::NW), 0, g.stream, t->d_codes,
-						   queries, t->kp, nrt, nqt, o);
-	}
+	if (o.nq > 128)
+		i8_tile_launch<4, KIND>(t, queries, o);
+	else if (o.nq > 64)
+		i8_tile_launch<2, KIND>(t, queries, o);
 	else
 		hipLaunchKernelGGL((k_i8_stream<2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
 						   nrb, nqb, o);
