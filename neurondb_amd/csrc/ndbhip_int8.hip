@@ -301,7 +301,8 @@ struct I8Out
 	int64_t		ostride;
 	int			ovec;			/* four scores may be stored at once */
 	float	   *gmax;			/* [nq][ngp]: the largest score of each block of 32 rows that takes part, -inf if none */
-	uint32_t	ngp;
+	float	   *qmax;			/* [nq][ngp / 4]: the largest of four blocks' */
+	uint32_t	ngp;			/* a multiple of 8; behind the last block of rows: not read */
 	uint32_t	n;
 	uint32_t	nq;
 };
@@ -438,13 +439,11 @@ template <int TB, class KIND>
 __global__ __launch_bounds__(256) void
 k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrb, uint32_t nqb, I8Out o)
 {
+	__shared__ __attribute__((aligned(16))) float s_m[KIND::MODE == 1 ? TB * 32 : 1][4];
 	const int	lane = threadIdx.x & 63;
 	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const uint32_t rb = blockIdx.x * 4 + wave;
+	const uint32_t rb = min(blockIdx.x * 4 + wave, nrb - 1);	/* (waves behind the last block do it over) */
 	const uint32_t qb0 = blockIdx.y * TB;
-
-	if (rb >= nrb)
-		return;
 	const unsigned char *a = rows + (size_t) rb * 32u * kp + lane * 16;
 	const unsigned char *b = queries + (size_t) qb0 * 32u * kp + lane * 16;
 	i8_v16i		acc[TB];
@@ -478,10 +477,26 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 																	 KIND::MASK ? i8_mask_word(o, rb, q) : 0u,
 																	 q < o.nq ? o.qscale[q] : 1.0f, acc[t]);
 
-				if (lane < 32 && q < o.nq)
-					o.gmax[(size_t) q * o.ngp + rb] = m;
+				if (lane < 32)
+					s_m[t * 32 + lane][wave] = m;
 			}
 		}
+	if (KIND::MODE == 1)
+	{
+		__syncthreads();
+		for (int i = threadIdx.x; i < TB * 32; i += 256)
+		{
+			const uint32_t q = qb0 * 32 + i;
+
+			if (q < o.nq)
+			{
+				const float4 m = *(const float4 *) s_m[i];
+
+				*(float4 *) (o.gmax + (size_t) q * o.ngp + blockIdx.x * 4) = m;
+				o.qmax[(size_t) q * (o.ngp / 4) + blockIdx.x] = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+			}
+		}
+	}
 }
 
 /* ------------------------------------------------------------------ */
@@ -728,7 +743,10 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 																KIND::MASK ? i8_mask_word(o, rb0 + i, q) : 0u,
 																q < o.nq ? qs : 1.0f, acc[i][t]);
 				if (q < o.nq && lane < 32)
+				{
 					*(float4 *) (o.gmax + (size_t) q * o.ngp + rb0) = make_float4(m[0], m[1], m[2], m[3]);
+					o.qmax[(size_t) q * (o.ngp / 4) + rb0 / 4] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+				}
 			}
 		}
 		slot = (slot + 1) & (I8_SLOTS - 1);
@@ -744,62 +762,252 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 /*
  * Any k best rows lie in the k row blocks with the largest maxima (equal maxima: the lower block first): a row of
  * another block has k rows ahead of it, one in each of those blocks.  So the product leaves one number per (query, 32
- * rows), k blocks are picked, and only their rows are scored again — one by one, with the same roundings.
+ * rows) and one per (query, four such blocks); k quads are picked, of their blocks k, and only the rows of those are scored
+ * again, one by one and with the same roundings.  The same holds at every step: the k-th of the maxima picked is a
+ * floor under the k-th best of what lies below them, so that a step looks at little more than k candidates.
  *
- * k_i8_pick: a block of threads per query; picked[q][0 .. npicked[q]) in ascending order.
+ * What is selected is ordered by one 64-bit word, larger scores first and then lower ids; all of them differ.
  */
-__global__ __launch_bounds__(256) void
-k_i8_pick(const float *__restrict__ gmax, uint32_t ngp, uint32_t ng, uint32_t k, uint32_t *__restrict__ picked, uint32_t *__restrict__ npicked)
+__device__ __forceinline__ uint64_t
+i8_word(float v, uint32_t id)
 {
-	__shared__ uint32_t hist[256], sh[16];
-	__shared__ uint64_t comp[NDBHIP_MAX_K];
-	__shared__ uint32_t pay[NDBHIP_MAX_K];
-	const uint32_t q = blockIdx.x;
-	const float *gm = gmax + (size_t) q * ngp;
-	auto		f = [&](uint32_t i, uint32_t &bits) -> bool {
-		const float m = gm[i];
+	return (uint64_t) ndb_key_from_bits(__float_as_uint(-v)) << 32 | id;
+}
+__device__ __forceinline__ float
+i8_word_score(uint64_t w)
+{
+	const uint32_t k = (uint32_t) (w >> 32);
 
-		bits = __float_as_uint(-m);
-		return m > I8_NINF;
-	};
-	uint32_t	T, less, kk, eq;
-
-	block_radix_select(f, ng, k, hist, sh, T, less, kk, eq);
-	if (threadIdx.x == 0)
-		npicked[q] = kk;
-	if (kk == 0)
-		return;
-	block_ordered_gather(f, ng, T, kk - less, sh, [&](int cls, uint32_t rank, uint32_t i, uint32_t) {
-		comp[cls == 0 ? rank : less + rank] = i;
-	});
-	__syncthreads();
-	uint32_t	npad = 1;
-
-	while (npad < kk)
-		npad <<= 1;
-	for (uint32_t i = kk + threadIdx.x; i < npad; i += blockDim.x)
-		comp[i] = ~0ull;
-	block_bitonic_sort(comp, pay, npad);
-	for (uint32_t i = threadIdx.x; i < kk; i += blockDim.x)
-		picked[(size_t) q * k + i] = (uint32_t) comp[i];
+	return -__uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k) + 0.0f;	/* (-0 and 0 are equal scores: 0) */
 }
 
-/* a wave per (query, picked block): lane l sums 16-byte pieces of row l % 32 against the query's, halves joined at the end */
-__global__ __launch_bounds__(256) void
-k_i8_rescore(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, I8Out o, uint32_t k,
-			 const uint32_t *__restrict__ picked, const uint32_t *__restrict__ npicked, float *__restrict__ cand)
+template <int NT, int CAP> struct I8Select
+{
+	uint64_t	list[CAP];
+	uint32_t	hist[256], sh[16];
+	float		top[NT];
+	float		floor;
+	uint32_t	cnt;
+};
+
+/* list[0 .. m) ascending; m <= CAP, a power of two.  Counting ranks beats the network's barriers for a few hundred words. */
+template <int NT, int CAP>
+__device__ void
+i8_sort(I8Select<NT, CAP> &S, uint32_t m)
+{
+	if (m <= 512)
+	{
+		uint64_t	v[(512 + NT - 1) / NT];
+		uint32_t	r[(512 + NT - 1) / NT];
+
+#pragma unroll
+		for (int e = 0; e < (512 + NT - 1) / NT; e++)
+			if (threadIdx.x + e * NT < m)
+			{
+				v[e] = S.list[threadIdx.x + e * NT];
+				r[e] = lds_rank_u64(S.list, m, v[e]);
+			}
+		__syncthreads();
+#pragma unroll
+		for (int e = 0; e < (512 + NT - 1) / NT; e++)
+			if (threadIdx.x + e * NT < m)
+				S.list[r[e]] = v[e];
+		__syncthreads();
+		return;
+	}
+	uint32_t	npad = 1024;
+
+	while (npad < m)
+		npad <<= 1;
+	for (uint32_t i = m + threadIdx.x; i < npad; i += NT)
+		S.list[i] = ~0ull;
+	for (uint32_t size = 2; size <= npad; size <<= 1)
+		for (uint32_t stride = size >> 1; stride > 0; stride >>= 1)
+		{
+			__syncthreads();
+			for (uint32_t t = threadIdx.x; t < (npad >> 1); t += NT)
+			{
+				const uint32_t lo = 2 * t - (t & (stride - 1)), hi = lo + stride;
+				const uint64_t x = S.list[lo], y = S.list[hi];
+
+				if ((x > y) == ((lo & size) == 0))
+				{
+					S.list[lo] = y;
+					S.list[hi] = x;
+				}
+			}
+		}
+	__syncthreads();
+}
+
+/*
+ * The min(k, valid) best of the elements f(i, score, id) -> takes part, i = 0 .. n - 1, in order in S.list; returns how
+ * many.  At least min(k, valid) elements have to reach `floor`.  Where more do than the list holds (many equal scores), the
+ * k-th score is found by radix selection, and the k-th id among its equals.  Ends with a barrier.
+ */
+template <int NT, int CAP, class F>
+__device__ uint32_t
+i8_select(I8Select<NT, CAP> &S, F f, uint32_t n, uint32_t k, float floor)
+{
+	if (threadIdx.x == 0)
+		S.cnt = 0;
+	__syncthreads();
+	for (uint32_t i = threadIdx.x; i < n; i += NT)
+	{
+		float		v;
+		uint32_t	id;
+
+		if (f(i, v, id) && v >= floor)
+		{
+			const uint32_t at = atomicAdd(&S.cnt, 1u);
+
+			if (at < CAP)
+				S.list[at] = i8_word(v, id);
+		}
+	}
+	__syncthreads();
+	uint32_t	m = S.cnt;
+
+	if (m > CAP)
+	{
+		uint32_t	T, less, kk, eq, T2 = ~0u;
+
+		block_radix_select([&](uint32_t i, uint32_t &bits) -> bool {
+			float		v;
+			uint32_t	id;
+			const bool	ok = f(i, v, id);
+
+			bits = __float_as_uint(-v);
+			return ok;
+		}, n, k, S.hist, S.sh, T, less, kk, eq);
+		if (eq > kk - less)
+		{
+			uint32_t	l2, k2, e2;
+
+			block_radix_select([&](uint32_t i, uint32_t &bits) -> bool {
+				float		v;
+				const bool	ok = f(i, v, bits);
+
+				return ok && ndb_key_from_bits(__float_as_uint(-v)) == T;
+			}, n, kk - less, S.hist, S.sh, T2, l2, k2, e2);
+		}
+		if (threadIdx.x == 0)
+			S.cnt = 0;
+		__syncthreads();
+		for (uint32_t i = threadIdx.x; i < n; i += NT)
+		{
+			float		v;
+			uint32_t	id;
+
+			if (!f(i, v, id))
+				continue;
+			const uint32_t key = ndb_key_from_bits(__float_as_uint(-v));
+
+			/* (ids are below 2^31: as keys of floats they keep their order) */
+			if (key < T || (key == T && ndb_key_from_bits(id) <= T2))
+				S.list[atomicAdd(&S.cnt, 1u)] = i8_word(v, id);
+		}
+		__syncthreads();
+		m = kk;
+	}
+	i8_sort(S, m);
+	return min(m, k);
+}
+
+/*
+ * The k best blocks of 32 rows of a query, in S.list; returns how many there are.  The floor of the first step: the
+ * k-th largest of the maxima of 2k .. 4k groups of threads' quads.
+ */
+template <int NT, int CAP>
+__device__ uint32_t
+i8_pick(I8Select<NT, CAP> &S, uint32_t *quads, const float *gm, const float *qm, uint32_t ng, uint32_t k)
+{
+	const uint32_t nquad = (ng + 3) / 4;
+	float		t = I8_NINF;
+	uint32_t	groups = NT / 64;
+
+	while (groups < 2 * k && groups < NT)
+		groups <<= 1;
+	for (uint32_t i = threadIdx.x; i < nquad; i += 8 * NT)
+	{
+		float		v[8];
+
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			v[e] = i + e * NT < nquad ? qm[i + e * NT] : I8_NINF;
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			t = fmaxf(t, v[e]);
+	}
+	for (uint32_t off = 1; off < NT / groups; off <<= 1)
+		t = fmaxf(t, __shfl_xor(t, off, 64));
+	if (threadIdx.x % (NT / groups) == 0)
+		S.top[threadIdx.x / (NT / groups)] = t;
+	if (threadIdx.x == 0)
+		S.floor = I8_NINF;
+	__syncthreads();
+	if (k <= groups && groups <= 256)
+	{
+		if (threadIdx.x < groups)
+		{
+			const float mine = S.top[threadIdx.x];
+			uint32_t	r = 0;
+
+			for (uint32_t j = 0; j < groups; j += 8)
+#pragma unroll
+				for (uint32_t e = 0; e < 8; e++)
+				{
+					const float o = S.top[j + e];
+
+					r += o > mine || (o == mine && j + e < threadIdx.x) ? 1u : 0u;
+				}
+			if (r == k - 1)
+				S.floor = mine;
+		}
+		__syncthreads();
+	}
+	else if (k <= groups)
+	{
+		uint32_t	T, less, kk, eq;
+
+		block_radix_select([&](uint32_t i, uint32_t &bits) -> bool {
+			bits = __float_as_uint(-S.top[i]);
+			return S.top[i] > I8_NINF;
+		}, groups, k, S.hist, S.sh, T, less, kk, eq);
+		if (threadIdx.x == 0 && kk == k)
+			S.floor = i8_word_score((uint64_t) T << 32);
+		__syncthreads();
+	}
+	const float floor = S.floor;
+	const uint32_t nq4 = i8_select(S, [&](uint32_t i, float &v, uint32_t &id) -> bool {
+		v = qm[i];
+		id = i;
+		return v > I8_NINF;
+	}, nquad, k, floor);
+	const float floor2 = nq4 == k ? i8_word_score(S.list[k - 1]) : I8_NINF;
+
+	for (uint32_t i = threadIdx.x; i < nq4; i += NT)
+		quads[i] = (uint32_t) S.list[i];
+	__syncthreads();
+	return i8_select(S, [&](uint32_t i, float &v, uint32_t &id) -> bool {
+		id = quads[i / 4] * 4 + i % 4;
+		v = id < ng ? gm[id] : I8_NINF;
+		return v > I8_NINF;
+	}, nq4 * 4, k, floor2);
+}
+
+/* the scores of the 32 rows of block rb for query q, one a lane in both halves of the wave: a lane sums 16-byte pieces of
+ * row l % 32 against the query's, the halves joined at the end; rows that take no part: -inf */
+__device__ __forceinline__ float
+i8_rescore(const unsigned char *rows, const unsigned char *queries, uint32_t kp, const I8Out &o, uint32_t rb, uint32_t q)
 {
 	const int	lane = threadIdx.x & 63;
-	const uint32_t slot = blockIdx.x * 4 + (threadIdx.x >> 6);
-	const uint32_t q = blockIdx.y;
-
-	if (slot >= npicked[q])
-		return;
-	const uint32_t rb = picked[(size_t) q * k + slot];
 	const unsigned char *a = rows + (size_t) rb * 32u * kp + lane * 16;
 	const unsigned char *b = queries + (size_t) (q >> 5) * 32u * kp + (q & 31) * 16 + (lane >> 5) * 512;
+	const uint32_t r = rb * 32 + (lane & 31);
 	int			s = 0;
 
+#pragma unroll 8
 	for (uint32_t e = 0; e < kp; e += 32)
 	{
 		const i8_v4i x = *(const i8_v4i *) (a + (size_t) e * 32);
@@ -810,68 +1018,112 @@ k_i8_rescore(const unsigned char *__restrict__ rows, const unsigned char *__rest
 			s = __builtin_amdgcn_sdot4(x[i], y[i], s, false);
 	}
 	s += __shfl_xor(s, 32, 64);
-	if (lane < 32)
-	{
-		const uint32_t r = rb * 32 + lane;
-		float		v = i8_score(s, o.rscale[r], o.qscale[q]);
 
-		if (o.bias && r < o.n)
-			v = v + o.bias[r];
-		if (!(v > I8_NINF) || (o.mask && !(o.mask[(int64_t) q * o.mask_stride + rb] >> lane & 1u)))
-			v = I8_NINF;
-		cand[((size_t) q * k + slot) * 32 + lane] = v + 0.0f;	/* (-0 and 0 are equal scores) */
+	float		v = i8_score(s, o.rscale[r], o.qscale[q]);
+
+	if (o.bias && r < o.n)
+		v = v + o.bias[r];
+	if (!(v > I8_NINF) || (o.mask && !(o.mask[(int64_t) q * o.mask_stride + rb] >> (lane & 31) & 1u)))
+		v = I8_NINF;
+	return v;
+}
+
+template <int NT>
+__device__ __forceinline__ void
+i8_results(const uint64_t *list, uint32_t m, uint32_t k, int64_t *ids, float *scores)
+{
+	for (uint32_t i = threadIdx.x; i < k; i += NT)
+	{
+		ids[i] = i < m ? (int64_t) (uint32_t) list[i] : -1;
+		scores[i] = i < m ? i8_word_score(list[i]) : I8_NINF;
 	}
 }
 
-/* the k best of a query's candidates, which lie in the order of their ids */
-__global__ __launch_bounds__(256) void
-k_i8_best(const float *__restrict__ cand, const uint32_t *__restrict__ picked, const uint32_t *__restrict__ npicked, uint32_t k,
-		  int64_t *__restrict__ ids, float *__restrict__ scores)
+/* up to this k one block of threads takes a query from its maxima to its results */
+#define I8_FUSED_K 128
+
+template <int NT>
+__global__ __launch_bounds__(NT) void
+k_i8_finish(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, I8Out o, uint32_t k,
+			int64_t *__restrict__ ids, float *__restrict__ scores)
 {
-	__shared__ uint32_t hist[256], sh[16];
-	__shared__ uint64_t comp[NDBHIP_MAX_K];
-	__shared__ uint32_t pay[NDBHIP_MAX_K];
+	__shared__ I8Select<NT, 512> S;
+	__shared__ uint32_t picked[I8_FUSED_K];
+	__shared__ float cand[I8_FUSED_K * 32];
+	const uint32_t q = blockIdx.x;
+	const uint32_t kk = i8_pick(S, picked, o.gmax + (size_t) q * o.ngp, o.qmax + (size_t) q * (o.ngp / 4), (o.n + 31) / 32, k);
+	const float floor = kk == k ? i8_word_score(S.list[k - 1]) : I8_NINF;
+
+	for (uint32_t i = threadIdx.x; i < kk; i += NT)
+		picked[i] = (uint32_t) S.list[i];
+	__syncthreads();
+	for (uint32_t slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); slot < kk; slot += NT / 64)
+	{
+		const float v = i8_rescore(rows, queries, kp, o, picked[slot], q);
+
+		if ((threadIdx.x & 63) < 32)
+			cand[slot * 32 + (threadIdx.x & 31)] = v;
+	}
+	__syncthreads();
+	const uint32_t m = i8_select(S, [&](uint32_t i, float &v, uint32_t &id) -> bool {
+		v = cand[i];
+		id = picked[i / 32] * 32 + i % 32;
+		return v > I8_NINF;
+	}, kk * 32, k, floor);
+
+	i8_results<NT>(S.list, m, k, ids + (size_t) q * k, scores + (size_t) q * k);
+}
+
+/* larger k: the rows of a query's blocks are scored by as many waves as there are blocks */
+#define I8_NT 1024
+
+__global__ __launch_bounds__(I8_NT) void
+k_i8_pick(I8Out o, uint32_t k, uint32_t *__restrict__ picked, uint32_t *__restrict__ npicked, float *__restrict__ floors)
+{
+	__shared__ I8Select<I8_NT, 2048> S;
+	__shared__ uint32_t quads[NDBHIP_MAX_K];
+	const uint32_t q = blockIdx.x;
+	const uint32_t kk = i8_pick(S, quads, o.gmax + (size_t) q * o.ngp, o.qmax + (size_t) q * (o.ngp / 4), (o.n + 31) / 32, k);
+
+	for (uint32_t i = threadIdx.x; i < kk; i += I8_NT)
+		picked[(size_t) q * k + i] = (uint32_t) S.list[i];
+	if (threadIdx.x == 0)
+	{
+		npicked[q] = kk;
+		floors[q] = kk == k ? i8_word_score(S.list[k - 1]) : I8_NINF;
+	}
+}
+
+__global__ __launch_bounds__(256) void
+k_i8_rescore(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, I8Out o, uint32_t k,
+			 const uint32_t *__restrict__ picked, const uint32_t *__restrict__ npicked, float *__restrict__ cand)
+{
+	const uint32_t slot = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const uint32_t q = blockIdx.y;
+
+	if (slot >= npicked[q])
+		return;
+	const float v = i8_rescore(rows, queries, kp, o, picked[(size_t) q * k + slot], q);
+
+	if ((threadIdx.x & 63) < 32)
+		cand[((size_t) q * k + slot) * 32 + (threadIdx.x & 31)] = v;
+}
+
+__global__ __launch_bounds__(I8_NT) void
+k_i8_best(const float *__restrict__ cand, const uint32_t *__restrict__ picked, const uint32_t *__restrict__ npicked,
+		  const float *__restrict__ floors, uint32_t k, int64_t *__restrict__ ids, float *__restrict__ scores)
+{
+	__shared__ I8Select<I8_NT, 2048> S;
 	const uint32_t q = blockIdx.x;
 	const float *c = cand + (size_t) q * k * 32;
-	const uint32_t n = npicked[q] * 32;
-	auto		f = [&](uint32_t i, uint32_t &bits) -> bool {
-		const float m = c[i];
+	const uint32_t *p = picked + (size_t) q * k;
+	const uint32_t m = i8_select(S, [&](uint32_t i, float &v, uint32_t &id) -> bool {
+		v = c[i];
+		id = p[i / 32] * 32 + i % 32;
+		return v > I8_NINF;
+	}, npicked[q] * 32, k, floors[q]);
 
-		bits = __float_as_uint(-m);
-		return m > I8_NINF;
-	};
-	uint32_t	T, less, kk, eq;
-
-	block_radix_select(f, n, k, hist, sh, T, less, kk, eq);
-	if (kk > 0)
-	{
-		block_ordered_gather(f, n, T, kk - less, sh, [&](int cls, uint32_t rank, uint32_t i, uint32_t bits) {
-			comp[cls == 0 ? rank : less + rank] = (uint64_t) ndb_key_from_bits(bits) << 32 | i;
-		});
-		__syncthreads();
-		uint32_t	npad = 1;
-
-		while (npad < kk)
-			npad <<= 1;
-		for (uint32_t i = kk + threadIdx.x; i < npad; i += blockDim.x)
-			comp[i] = ~0ull;
-		block_bitonic_sort(comp, pay, npad);
-	}
-	for (uint32_t i = threadIdx.x; i < k; i += blockDim.x)
-	{
-		int64_t		id = -1;
-		float		s = I8_NINF;
-
-		if (i < kk)
-		{
-			const uint32_t at = (uint32_t) comp[i];
-
-			id = (int64_t) picked[(size_t) q * k + at / 32] * 32 + at % 32;
-			s = c[at];
-		}
-		ids[(size_t) q * k + i] = id;
-		scores[(size_t) q * k + i] = s;
-	}
+	i8_results<I8_NT>(S.list, m, k, ids + (size_t) q * k, scores + (size_t) q * k);
 }
 
 __global__ __launch_bounds__(256) void
@@ -1322,7 +1574,7 @@ i8_round(size_t b)
 struct I8Ws
 {
 	uint32_t	nqp, ng, ngp;
-	size_t		q_off, qs_off, gm_off, pick_off, npick_off, cand_off, total;
+	size_t		q_off, qs_off, gm_off, qm_off, pick_off, npick_off, floor_off, cand_off, total;
 };
 
 static I8Ws
@@ -1338,9 +1590,13 @@ i8_ws(const ndbhip_i8 *t, int nq, int k)
 	w.q_off = take((size_t) w.nqp * t->kp);
 	w.qs_off = take((size_t) w.nqp * sizeof(float));
 	w.gm_off = take(k ? (size_t) nq * w.ngp * sizeof(float) : 0);
-	w.pick_off = take((size_t) nq * k * sizeof(uint32_t));
-	w.npick_off = take(k ? (size_t) nq * sizeof(uint32_t) : 0);
-	w.cand_off = take((size_t) nq * k * 32 * sizeof(float));
+	w.qm_off = take(k ? (size_t) nq * (w.ngp / 4) * sizeof(float) : 0);
+	const size_t split = k > I8_FUSED_K ? (size_t) nq : 0;
+
+	w.pick_off = take(split * k * sizeof(uint32_t));
+	w.npick_off = take(split * sizeof(uint32_t));
+	w.floor_off = take(split * sizeof(float));
+	w.cand_off = take(split * k * 32 * sizeof(float));
 	w.total = at;
 	return w;
 }
@@ -1349,7 +1605,7 @@ i8_ws(const ndbhip_i8 *t, int nq, int k)
 static int
 i8_chunk(const ndbhip_i8 *t, int nq, int k)
 {
-	const size_t per = (size_t) t->kp + (size_t) (t->n + 255) / 8 + (size_t) k * 132 + 8;
+	const size_t per = (size_t) t->kp + (size_t) (t->n + 255) / 32 * 5 + (k > I8_FUSED_K ? (size_t) k * 132 : 0) + 12;
 	const int64_t m = std::max<int64_t>(256, (int64_t) (((size_t) 1 << 30) / per) / 256 * 256);
 
 	return (int) std::min<int64_t>(nq, std::min<int64_t>(m, 4096));
@@ -1538,7 +1794,7 @@ ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const f
 		char	   *ws = (char *) d_ws;
 		const unsigned char *qc = (const unsigned char *) ws + w.q_off;
 		uint32_t   *picked = (uint32_t *) (ws + w.pick_off), *npicked = (uint32_t *) (ws + w.npick_off);
-		float	   *cand = (float *) (ws + w.cand_off);
+		float	   *floors = (float *) (ws + w.floor_off), *cand = (float *) (ws + w.cand_off);
 		I8Out		o = {};
 
 		if ((rc = i8_take_queries(t, d_q, q_type, d_q_scales, q0, m, q_stride, ws, w)))
@@ -1549,16 +1805,26 @@ ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const f
 		o.mask = d_mask ? d_mask + q0 * mask_stride : nullptr;
 		o.mask_stride = mask_stride;
 		o.gmax = (float *) (ws + w.gm_off);
+		o.qmax = (float *) (ws + w.qm_off);
 		o.ngp = w.ngp;
 		o.n = (uint32_t) t->n;
 		o.nq = (uint32_t) m;
 		if ((rc = i8_multiply_maxima(t, qc, o)))
 			return rc;
-		hipLaunchKernelGGL(k_i8_pick, dim3(m), dim3(256), 0, g.stream, o.gmax, w.ngp, w.ng, (uint32_t) k, picked, npicked);
-		hipLaunchKernelGGL(k_i8_rescore, dim3((k + 3) / 4, m), dim3(256), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, picked,
-						   npicked, cand);
-		hipLaunchKernelGGL(k_i8_best, dim3(m), dim3(256), 0, g.stream, cand, picked, npicked, (uint32_t) k, d_ids + q0 * k,
-						   d_scores + q0 * k);
+		if (k > I8_FUSED_K)
+		{
+			hipLaunchKernelGGL(k_i8_pick, dim3(m), dim3(I8_NT), 0, g.stream, o, (uint32_t) k, picked, npicked, floors);
+			hipLaunchKernelGGL(k_i8_rescore, dim3((k + 3) / 4, m), dim3(256), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, picked,
+							   npicked, cand);
+			hipLaunchKernelGGL(k_i8_best, dim3(m), dim3(I8_NT), 0, g.stream, cand, picked, npicked, floors, (uint32_t) k, d_ids + q0 * k,
+							   d_scores + q0 * k);
+		}
+		else if (m < g.num_cus)
+			hipLaunchKernelGGL(k_i8_finish<1024>, dim3(m), dim3(1024), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, d_ids + q0 * k,
+							   d_scores + q0 * k);
+		else
+			hipLaunchKernelGGL(k_i8_finish<256>, dim3(m), dim3(256), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, d_ids + q0 * k,
+							   d_scores + q0 * k);
 		HIP_TRY(hipGetLastError());
 	}
 	NDB_STAT_ADD(queries, nq);
