@@ -199,12 +199,13 @@ k_i8_quantize(const T *__restrict__ x, int64_t nrows, int64_t nrows_out, int dim
 		}
 }
 
-/* byte * scale in fp32, rounded once more where the output has 16 bits; a thread takes four elements */
+/* byte * scale in fp32, rounded once more where the output has 16 bits; a lane takes four elements at a time, CH loads ahead */
 template <class T>
 __global__ __launch_bounds__(256) void
 k_i8_dequantize(const int8_t *__restrict__ codes, int64_t cstride, int cvec, const float *__restrict__ scales, int64_t nrows, int dim,
 				int lanes_log2, T *__restrict__ out, int64_t ostride, int ovec)
 {
+	constexpr int CH = 4;
 	const int	L = 1 << lanes_log2;
 	const int	lane = threadIdx.x & (L - 1);
 	const int64_t row = (int64_t) blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2);
@@ -215,28 +216,40 @@ k_i8_dequantize(const int8_t *__restrict__ codes, int64_t cstride, int cvec, con
 	T		   *o = out + row * ostride;
 	const float s = scales[row];
 
-	for (int e = lane * 4; e < dim; e += 4 * L)
+	for (int e0 = lane * 4; e0 < dim; e0 += 4 * L * CH)
 	{
-		const int	m = min(4, dim - e);
-		uint32_t	w = 0;
-		I8Vec<T, 4> v;
+		uint32_t	w[CH];
 
-		if (cvec && m == 4)
-			w = *(const uint32_t *) (c + e);
-		else
+#pragma unroll
+		for (int u = 0; u < CH; u++)
+		{
+			const int	e = e0 + u * 4 * L;
+
+			w[u] = 0;
+			if (cvec && e + 4 <= dim)
+				w[u] = *(const uint32_t *) (c + e);
+			else
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					w[u] |= e + i < dim ? (uint32_t) (uint8_t) c[e + i] << (8 * i) : 0u;
+		}
+#pragma unroll
+		for (int u = 0; u < CH; u++)
+		{
+			const int	e = e0 + u * 4 * L;
+			I8Vec<T, 4> v;
+
 #pragma unroll
 			for (int i = 0; i < 4; i++)
-				w |= i < m ? (uint32_t) (uint8_t) c[e + i] << (8 * i) : 0u;
+				v.v[i] = I8Elem<T>::store((float) (int8_t) (w[u] >> (8 * i)) * s);
+			if (ovec && e + 4 <= dim)
+				*(I8Vec<T, 4> *) (o + e) = v;
+			else
 #pragma unroll
-		for (int i = 0; i < 4; i++)
-			v.v[i] = I8Elem<T>::store((float) (int8_t) (w >> (8 * i)) * s);
-		if (ovec && m == 4)
-			*(I8Vec<T, 4> *) (o + e) = v;
-		else
-#pragma unroll
-			for (int i = 0; i < 4; i++)
-				if (i < m)
-					o[e + i] = v.v[i];
+				for (int i = 0; i < 4; i++)
+					if (e + i < dim)
+						o[e + i] = v.v[i];
+		}
 	}
 }
 
@@ -316,7 +329,7 @@ i8_score(int dot, float rs, float qs)
 
 /*
  * The block of sums of a row block rb and a query block: lane l has query l % 32 of it and, in register 4 g + j, row
- * 8 g + 4 (l / 32) + j.  rs, bias: from the row block's first on, in memory or in LDS; rows behind the last have a scale but no bias.
+ * 8 g + 4 (l / 32) + j.  rs, bias: from the row block's first on, in LDS.
  */
 template <bool BIAS, class T>
 __device__ __forceinline__ void
@@ -327,7 +340,6 @@ i8_write_scores(const I8Out &o, const float *rs, const float *bias, uint32_t rb,
 
 	if (q >= o.nq || rb * 32 >= o.n)
 		return;
-	const uint32_t left = o.n - rb * 32;
 	T		   *out = (T *) o.out + (int64_t) q * o.ostride;
 
 #pragma unroll
@@ -337,13 +349,14 @@ i8_write_scores(const I8Out &o, const float *rs, const float *bias, uint32_t rb,
 		const float4 r4 = *(const float4 *) (rs + 8 * g4 + 4 * h);
 		float		s[4] = {i8_score(acc[4 * g4], r4.x, qs), i8_score(acc[4 * g4 + 1], r4.y, qs),
 			i8_score(acc[4 * g4 + 2], r4.z, qs), i8_score(acc[4 * g4 + 3], r4.w, qs)};
+		const float4 b4 = BIAS ? *(const float4 *) (bias + 8 * g4 + 4 * h) : make_float4(0, 0, 0, 0);
 		I8Vec<T, 4> v;
 
 #pragma unroll
 		for (int j = 0; j < 4; j++)
 		{
 			if (BIAS)
-				s[j] = s[j] + bias[min((uint32_t) (8 * g4 + 4 * h + j), left - 1)];
+				s[j] = s[j] + (&b4.x)[j];
 			v.v[j] = I8Elem<T>::store(s[j]);
 		}
 		if (o.ovec && r + 4 <= o.n)
@@ -358,13 +371,13 @@ i8_write_scores(const I8Out &o, const float *rs, const float *bias, uint32_t rb,
 
 /*
  * The largest score that takes part among the 32 rows of block rb, for the lane's query (both halves of the wave hold it).
- * rs: the block's 32 row scales; bias: its nbias (1 .. 32) biases, padding rows have none.  fmaxf drops NaN: rows of NaN scores, padding rows among them, never take
+ * rs, bias: the block's 32 row scales and biases (in LDS).  fmaxf drops NaN: rows of NaN scores, padding rows among them, never take
  * part.  A product with a positive finite query scale rises with its other factor and so does its rounding, hence without
  * a bias RN(t * qs) is taken of the largest t only.
  */
 template <bool BIAS, bool MASK>
 __device__ __forceinline__ float
-i8_block_max(const float *rs, const float *bias, uint32_t nbias, uint32_t bits, float qs, const i8_v16i &acc)
+i8_block_max(const float *rs, const float *bias, uint32_t bits, float qs, const i8_v16i &acc)
 {
 	const int	h = (threadIdx.x & 63) >> 5;
 	const bool	rises = qs > 0.0f && qs < __builtin_inff();
@@ -400,6 +413,8 @@ i8_block_max(const float *rs, const float *bias, uint32_t nbias, uint32_t bits, 
 		{
 			const float4 r4 = *(const float4 *) (rs + 8 * g4 + 4 * h);
 			const float rv[4] = {r4.x, r4.y, r4.z, r4.w};
+			const float4 b4 = BIAS ? *(const float4 *) (bias + 8 * g4 + 4 * h) : make_float4(0, 0, 0, 0);
+			const float bv[4] = {b4.x, b4.y, b4.z, b4.w};
 
 #pragma unroll
 			for (int j = 0; j < 4; j++)
@@ -407,7 +422,7 @@ i8_block_max(const float *rs, const float *bias, uint32_t nbias, uint32_t bits, 
 				float		t = i8_score(acc[4 * g4 + j], rv[j], qs);
 
 				if (BIAS)
-					t = t + bias[min((uint32_t) (8 * g4 + 4 * h + j), nbias - 1)];
+					t = t + bv[j];
 				if (MASK)
 				{
 					const uint32_t in = (uint32_t) __builtin_amdgcn_sbfe((int) (bits >> (4 * h)), 8 * g4 + j, 1);
@@ -434,53 +449,85 @@ template <int MODE_, bool BIAS_, bool MASK_, class T_> struct I8Kind
 	typedef T_	T;
 };
 
-/* Few queries: a wave multiplies one block of 32 rows with TB blocks of 32 queries straight from memory. */
+/*
+ * Few queries: a wave multiplies one block of 32 rows with TB blocks of 32 queries straight from memory, U steps of 32
+ * dimensions requested at a time; the queries stay in the caches.  What the sums are combined with is requested first.
+ * Bound by HBM: the table is read once for every TB * 32 queries.
+ */
 template <int TB, class KIND>
 __global__ __launch_bounds__(256) void
-k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrb, uint32_t nqb, I8Out o)
+k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrb, I8Out o)
 {
+	constexpr int U = TB == 1 ? 8 : 4;
 	__shared__ __attribute__((aligned(16))) float s_m[KIND::MODE == 1 ? TB * 32 : 1][4];
+	__shared__ __attribute__((aligned(16))) float s_rs[4][32], s_bias[KIND::BIAS ? 4 : 1][32];
 	const int	lane = threadIdx.x & 63;
 	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const uint32_t rb = min(blockIdx.x * 4 + wave, nrb - 1);	/* (waves behind the last block do it over) */
 	const uint32_t qb0 = blockIdx.y * TB;
 	const unsigned char *a = rows + (size_t) rb * 32u * kp + lane * 16;
 	const unsigned char *b = queries + (size_t) qb0 * 32u * kp + lane * 16;
+	const uint32_t row = rb * 32 + (lane & 31);
+	const float my_rs = o.rscale[row];
+	const float my_bias = KIND::BIAS && row < o.n ? o.bias[row] : 0.0f;
+	float		qs[TB];
+	uint32_t	bits[TB];
 	i8_v16i		acc[TB];
 
 #pragma unroll
 	for (int t = 0; t < TB; t++)
+	{
+		const uint32_t q = (qb0 + t) * 32 + (lane & 31);
+
+		qs[t] = q < o.nq ? o.qscale[q] : 1.0f;
+		bits[t] = KIND::MASK ? i8_mask_word(o, rb, q) : 0u;
 #pragma unroll
 		for (int i = 0; i < 16; i++)
 			acc[t][i] = 0;
-	for (uint32_t k = 0; k < kp; k += 32)
-	{
-		const i8_v4i av = *(const i8_v4i *) (a + (size_t) k * 32);
-
-#pragma unroll
-		for (int t = 0; t < TB; t++)
-			if (qb0 + t < nqb)
-				acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, *(const i8_v4i *) (b + (size_t) t * 32 * kp + (size_t) k * 32),
-															   acc[t], 0, 0, 0);
 	}
+	for (uint32_t k = 0; k < kp; k += 32 * U)
+	{
+		i8_v4i		av[U], bv[U][TB];
+
+		/* (a step behind the last one asks for that one again and is not multiplied) */
+#pragma unroll
+		for (int u = 0; u < U; u++)
+			av[u] = *(const i8_v4i *) (a + (size_t) min(k + u * 32, kp - 32) * 32);
+#pragma unroll
+		for (int u = 0; u < U; u++)
+#pragma unroll
+			for (int t = 0; t < TB; t++)
+				bv[u][t] = *(const i8_v4i *) (b + (size_t) t * 32 * kp + (size_t) min(k + u * 32, kp - 32) * 32);
+#pragma unroll
+		for (int u = 0; u < U; u++)
+			if (k + u * 32 < kp)
+#pragma unroll
+				for (int t = 0; t < TB; t++)
+					acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[u], bv[u][t], acc[t], 0, 0, 0);
+	}
+	/* (a wave's own LDS: what it writes it reads in order) */
+	if (lane < 32)
+	{
+		s_rs[wave][lane] = my_rs;
+		if (KIND::BIAS)
+			s_bias[wave][lane] = my_bias;
+	}
+	__builtin_amdgcn_wave_barrier();
 #pragma unroll
 	for (int t = 0; t < TB; t++)
-		if (qb0 + t < nqb)
+	{
+		const uint32_t q = (qb0 + t) * 32 + (lane & 31);
+
+		if (KIND::MODE == 0)
+			i8_write_scores<KIND::BIAS, typename KIND::T>(o, s_rs[wave], s_bias[KIND::BIAS ? wave : 0], rb, q, qs[t], acc[t]);
+		else
 		{
-			const uint32_t q = (qb0 + t) * 32 + (lane & 31);
+			const float m = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs[wave], s_bias[KIND::BIAS ? wave : 0], bits[t], qs[t], acc[t]);
 
-			if (KIND::MODE == 0)
-				i8_write_scores<KIND::BIAS, typename KIND::T>(o, o.rscale + rb * 32, o.bias + rb * 32, rb, q, o.qscale[q], acc[t]);
-			else
-			{
-				const float m = i8_block_max<KIND::BIAS, KIND::MASK>(o.rscale + rb * 32, o.bias + rb * 32, min(32u, o.n - rb * 32),
-																	 KIND::MASK ? i8_mask_word(o, rb, q) : 0u,
-																	 q < o.nq ? o.qscale[q] : 1.0f, acc[t]);
-
-				if (lane < 32)
-					s_m[t * 32 + lane][wave] = m;
-			}
+			if (lane < 32)
+				s_m[t * 32 + lane][wave] = m;
 		}
+	}
 	if (KIND::MODE == 1)
 	{
 		__syncthreads();
@@ -739,7 +786,7 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 #pragma unroll
 				for (int i = 0; i < 4; i++)
 					m[i] = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs[slot] + (wr * 4 + i) * 32,
-																s_bias[KIND::BIAS ? slot : 0] + (wr * 4 + i) * 32, 32u,
+																s_bias[KIND::BIAS ? slot : 0] + (wr * 4 + i) * 32,
 																KIND::MASK ? i8_mask_word(o, rb0 + i, q) : 0u,
 																q < o.nq ? qs : 1.0f, acc[i][t]);
 				if (q < o.nq && lane < 32)
@@ -1039,8 +1086,12 @@ i8_results(const uint64_t *list, uint32_t m, uint32_t k, int64_t *ids, float *sc
 	}
 }
 
-/* up to this k one block of threads takes a query from its maxima to its results */
+/*
+ * One block of threads takes a query from its maxima to its results where its candidates fit LDS (k <= 128) and either
+ * there are blocks for the whole chip or a query's picked rows are few bytes: a lone block reads about 60 GB/s.
+ */
 #define I8_FUSED_K 128
+#define I8_FUSED_BYTES (512u << 10)
 
 template <int NT>
 __global__ __launch_bounds__(NT) void
@@ -1143,21 +1194,57 @@ k_i8_none(int64_t *__restrict__ ids, float *__restrict__ scores, uint64_t n)
 /* ================================================================== */
 
 /*
- * A block of threads takes COLS columns of one query: counts how often the query's list names each of them (the whole
- * list is read per block: it is short next to the columns, and LDS counters need neither a sort nor a hash nor a bound
- * on its length), then passes over the scores once.  Bound by HBM: a score read and written, a bit of mask.
+ * A block of threads takes 256 * VEC * U neighbouring columns of one query and reads their scores at once; meanwhile it counts how
+ * often the query's list names each of them (the whole list is read per block: it is short next to the columns, and
+ * LDS counters need neither a sort nor a hash nor a bound on its length).  Bound by HBM: a score read and written, a bit
+ * of mask.
  */
-template <class T>
+template <class T, int U>
 __global__ __launch_bounds__(256) void
-k_scores_adjust(const T *scores, int64_t stride, int64_t n, int cols, int svec, const int64_t *__restrict__ seen_off,
+k_scores_adjust(const T *scores, int64_t stride, int64_t n, int svec, const int64_t *__restrict__ seen_off,
 				const int32_t *__restrict__ seen_ids, const float *__restrict__ penalties, const float *__restrict__ bias, int64_t bias_stride,
-				const uint32_t *__restrict__ mask, int64_t mask_stride, T *out, int64_t ostride, int q0)
+				int bvec, const uint32_t *__restrict__ mask, int64_t mask_stride, T *out, int64_t ostride, int q0)
 {
-	constexpr int VEC = 16 / sizeof(T);
-	extern __shared__ uint32_t cnt[];
+	constexpr int VEC = 16 / sizeof(T), COLS = 256 * VEC * U;
+	__shared__ __attribute__((aligned(16))) uint32_t cnt[COLS];
 	const int64_t q = q0 + blockIdx.y;
-	const int64_t c0 = (int64_t) blockIdx.x * cols;
-	const int	m = (int) min((int64_t) cols, n - c0);
+	const int64_t c0 = (int64_t) blockIdx.x * COLS;
+	const int	m = (int) min((int64_t) COLS, n - c0);
+	const T    *src = scores + q * stride + c0;
+	T		   *dst = out + q * ostride + c0;
+	const float *bv = bias ? bias + q * bias_stride + c0 : nullptr;
+	const uint32_t *mv = mask ? mask + q * mask_stride + c0 / 32 : nullptr;
+	I8Vec<T, VEC> v[U];
+	float		add[U][VEC];
+	uint32_t	word[U];
+
+#pragma unroll
+	for (int u = 0; u < U; u++)
+	{
+		const int	e = (u * 256 + threadIdx.x) * VEC;
+
+		word[u] = 0xFFFFFFFFu;
+		if (e < m)
+		{
+			if (svec && e + VEC <= m)
+				v[u] = *(const I8Vec<T, VEC> *) (src + e);
+			else
+#pragma unroll
+				for (int i = 0; i < VEC; i++)
+					if (e + i < m)
+						v[u].v[i] = src[e + i];
+			if (mv)
+				word[u] = mv[e / 32] >> (e % 32);
+			if (bv && bvec && e + VEC <= m)
+#pragma unroll
+				for (int i = 0; i < VEC; i += 4)
+					*(float4 *) &add[u][i] = *(const float4 *) (bv + e + i);
+			else if (bv)
+#pragma unroll
+				for (int i = 0; i < VEC; i++)
+					add[u][i] = e + i < m ? bv[e + i] : 0.0f;
+		}
+	}
 	const int64_t lo = seen_off ? seen_off[q] : 0, hi = seen_off ? seen_off[q + 1] : 0;
 	const bool	seen = hi > lo;
 	float		repeat = 1.0f, presence = 0.0f, frequency = 0.0f;
@@ -1167,8 +1254,8 @@ k_scores_adjust(const T *scores, int64_t stride, int64_t n, int cols, int svec, 
 		repeat = penalties[3 * q];
 		presence = penalties[3 * q + 1];
 		frequency = penalties[3 * q + 2];
-		for (int i = threadIdx.x; i < m; i += 256)
-			cnt[i] = 0;
+		for (int i = threadIdx.x * 4; i < COLS; i += 1024)
+			*(uint4 *) &cnt[i] = make_uint4(0, 0, 0, 0);
 		__syncthreads();
 		for (int64_t i = lo + threadIdx.x; i < hi; i += 256)
 		{
@@ -1179,49 +1266,54 @@ k_scores_adjust(const T *scores, int64_t stride, int64_t n, int cols, int svec, 
 		}
 		__syncthreads();
 	}
-	const T    *src = scores + q * stride + c0;
-	T		   *dst = out + q * ostride + c0;
-	const float *bv = bias ? bias + q * bias_stride + c0 : nullptr;
-	const uint32_t *mv = mask ? mask + q * mask_stride + c0 / 32 : nullptr;
-
-	for (int e = threadIdx.x * VEC; e < m; e += 256 * VEC)
-	{
-		I8Vec<T, VEC> v;
-		const bool	whole = svec && e + VEC <= m;
-		const uint32_t word = mv ? mv[e / 32] >> (e % 32) : 0xFFFFFFFFu;
-
-		if (whole)
-			v = *(const I8Vec<T, VEC> *) (src + e);
-		else
 #pragma unroll
-			for (int i = 0; i < VEC; i++)
-				if (e + i < m)
-					v.v[i] = src[e + i];
+	for (int u = 0; u < U; u++)
+	{
+		const int	e = (u * 256 + threadIdx.x) * VEC;
+
+		if (e >= m)
+			break;
+		uint32_t	c[VEC], any = 0;
+
 #pragma unroll
 		for (int i = 0; i < VEC; i++)
-			if (e + i < m)
+			c[i] = 0;
+		if (seen)
+#pragma unroll
+			for (int i = 0; i < VEC; i += 4)
 			{
-				float		s = I8Elem<T>::load(v.v[i]);
-				const uint32_t c = seen ? cnt[e + i] : 0u;
-
-				if (c > 0)
-				{
-					s = s > 0.0f ? s / repeat : s * repeat;
-					s = s - (presence + (float) c * frequency);
-				}
-				if (bv)
-					s = s + bv[e + i];
-				if (!(word >> i & 1u))
-					s = I8_NINF;
-				v.v[i] = I8Elem<T>::store(s);
+				*(uint4 *) &c[i] = *(const uint4 *) &cnt[e + i];
+				any |= c[i] | c[i + 1] | c[i + 2] | c[i + 3];
 			}
-		if (whole)
-			*(I8Vec<T, VEC> *) (dst + e) = v;
+		float		s[VEC];
+
+#pragma unroll
+		for (int i = 0; i < VEC; i++)
+			s[i] = I8Elem<T>::load(v[u].v[i]);
+		if (any)
+#pragma unroll
+			for (int i = 0; i < VEC; i++)
+				if (c[i] > 0)
+				{
+					s[i] = s[i] > 0.0f ? s[i] / repeat : s[i] * repeat;
+					s[i] = s[i] - (presence + (float) c[i] * frequency);
+				}
+#pragma unroll
+		for (int i = 0; i < VEC; i++)
+		{
+			if (bv)
+				s[i] = s[i] + add[u][i];
+			if (!(word[u] >> i & 1u))
+				s[i] = I8_NINF;
+			v[u].v[i] = I8Elem<T>::store(s[i]);
+		}
+		if (svec && e + VEC <= m)
+			*(I8Vec<T, VEC> *) (dst + e) = v[u];
 		else
 #pragma unroll
 			for (int i = 0; i < VEC; i++)
 				if (e + i < m)
-					dst[e + i] = v.v[i];
+					dst[e + i] = v[u].v[i];
 	}
 }
 
@@ -1577,6 +1669,12 @@ struct I8Ws
 	size_t		q_off, qs_off, gm_off, qm_off, pick_off, npick_off, floor_off, cand_off, total;
 };
 
+static bool
+i8_fused(const ndbhip_i8 *t, int nq, int k)
+{
+	return k <= I8_FUSED_K && (nq >= g.num_cus || (uint64_t) k * 32 * t->kp <= I8_FUSED_BYTES);
+}
+
 static I8Ws
 i8_ws(const ndbhip_i8 *t, int nq, int k)
 {
@@ -1591,7 +1689,8 @@ i8_ws(const ndbhip_i8 *t, int nq, int k)
 	w.qs_off = take((size_t) w.nqp * sizeof(float));
 	w.gm_off = take(k ? (size_t) nq * w.ngp * sizeof(float) : 0);
 	w.qm_off = take(k ? (size_t) nq * (w.ngp / 4) * sizeof(float) : 0);
-	const size_t split = k > I8_FUSED_K ? (size_t) nq : 0;
+	/* (what ndbhip_i8_workspace says grows with nq: room for the largest batch that is not fused) */
+	const size_t split = k > I8_FUSED_K ? (size_t) nq : i8_fused(t, 1, k) ? 0 : (size_t) std::min(nq, g.num_cus);
 
 	w.pick_off = take(split * k * sizeof(uint32_t));
 	w.npick_off = take(split * sizeof(uint32_t));
@@ -1683,8 +1782,13 @@ i8_multiply_kind(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &
 	else if (o.nq > 64)
 		i8_tile_launch<2, KIND>(t, queries, o);
 	else
-		hipLaunchKernelGGL((k_i8_stream<2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
-						   nrb, nqb, o);
+	{
+		if (nqb == 1)
+			hipLaunchKernelGGL((k_i8_stream<1, KIND>), dim3((nrb + 3) / 4), dim3(256), 0, g.stream, t->d_codes, queries, t->kp, nrb, o);
+		else
+			hipLaunchKernelGGL((k_i8_stream<2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
+							   nrb, o);
+	}
 	HIP_TRY(hipGetLastError());
 	return NDBHIP_OK;
 }
@@ -1811,7 +1915,7 @@ ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const f
 		o.nq = (uint32_t) m;
 		if ((rc = i8_multiply_maxima(t, qc, o)))
 			return rc;
-		if (k > I8_FUSED_K)
+		if (!i8_fused(t, m, k))
 		{
 			hipLaunchKernelGGL(k_i8_pick, dim3(m), dim3(I8_NT), 0, g.stream, o, (uint32_t) k, picked, npicked, floors);
 			hipLaunchKernelGGL(k_i8_rescore, dim3((k + 3) / 4, m), dim3(256), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, picked,
@@ -1894,13 +1998,23 @@ static void
 scores_adjust_launch(const void *s, int64_t stride, int nq, int64_t n, const int64_t *off, const int32_t *ids, const float *pen, const float *bias,
 					 int64_t bias_stride, const uint32_t *mask, int64_t mask_stride, void *out, int64_t ostride)
 {
-	const int	cols = (int64_t) nq * n >= ((int64_t) 8 << 20) ? 8192 : 2048;
+	/* columns a block takes: many scores 4096 (fp32) or 8192 (16 bits), which halves the list's reads; else half of that */
+	constexpr int VEC = 16 / sizeof(T);
+	const int	u = (int64_t) nq * n >= ((int64_t) 4 << 20) ? 4 : 2, cols = 256 * VEC * u;
 	const int	vec = i8_aligned(s, stride * (int64_t) sizeof(T), 16) && i8_aligned(out, ostride * (int64_t) sizeof(T), 16);
+	const int	bvec = i8_aligned(bias, bias_stride * 4, 16);
 
 	for (int q0 = 0; q0 < nq; q0 += 65535)
-		hipLaunchKernelGGL(k_scores_adjust<T>, dim3((unsigned) ((n + cols - 1) / cols), std::min(65535, nq - q0)), dim3(256),
-						   off ? cols * sizeof(uint32_t) : 0, g.stream, (const T *) s, stride, n, cols, vec, off, ids, pen, bias, bias_stride,
-						   mask, mask_stride, (T *) out, ostride, q0);
+	{
+		const dim3	grid((unsigned) ((n + cols - 1) / cols), std::min(65535, nq - q0));
+
+		if (u == 4)
+			hipLaunchKernelGGL((k_scores_adjust<T, 4>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, vec, off, ids, pen, bias,
+							   bias_stride, bvec, mask, mask_stride, (T *) out, ostride, q0);
+		else
+			hipLaunchKernelGGL((k_scores_adjust<T, 2>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, vec, off, ids, pen, bias,
+							   bias_stride, bvec, mask, mask_stride, (T *) out, ostride, q0);
+	}
 }
 
 extern "C" int
