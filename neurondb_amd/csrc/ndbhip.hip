@@ -327,7 +327,8 @@ ndbhip_set_thread_stream(void *s)
 extern "C" int
 ndbhip_swap_thread_stream(void *s, void **prev)
 {
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	if (!g.inited)			/* (nothing is launched here: the current device may be any) */
+		return fail(NDBHIP_ERR_NODEVICE, "ndbhip_init() has not succeeded in this process");
 	if (!prev)
 		return fail(NDBHIP_ERR_INVALID, "out is NULL");
 	*prev = (void *) ndbhip_tl_stream;

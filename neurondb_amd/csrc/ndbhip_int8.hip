@@ -312,7 +312,6 @@ struct I8Out
 	int64_t		mask_stride;	/* words from one query to the next; 0 = one mask for all */
 	void	   *out;			/* scores */
 	int64_t		ostride;
-	int			ovec;			/* four scores may be stored at once */
 	float	   *gmax;			/* [nq][ngp]: the largest score of each block of 32 rows that takes part, -inf if none */
 	float	   *qmax;			/* [nq][ngp / 4]: the largest of four blocks' */
 	uint32_t	ngp;			/* a multiple of 8; behind the last block of rows: not read */
@@ -328,49 +327,50 @@ i8_score(int dot, float rs, float qs)
 }
 
 /*
- * The block of sums of a row block rb and a query block: lane l has query l % 32 of it and, in register 4 g + j, row
- * 8 g + 4 (l / 32) + j.  rs, bias: from the row block's first on, in LDS.
+ * Writes the block of sums of row block rb and the query block that starts at query q0.  The matrix instruction had the
+ * queries as its first operand: lane l has row l % 32 and, in register 4 g + j, query 8 g + 4 (l / 32) + j, so that a store
+ * covers 32 neighbouring scores of each of two queries, whatever the matrix's alignment.  rs, bias: of the lane's row;
+ * qs: the block's 32 query scales, in LDS.
  */
 template <bool BIAS, class T>
 __device__ __forceinline__ void
-i8_write_scores(const I8Out &o, const float *rs, const float *bias, uint32_t rb, uint32_t q, float qs, const i8_v16i &acc)
+i8_write_scores(const I8Out &o, float rs, float bias, const float *qs, uint32_t rb, uint32_t q0, const i8_v16i &acc)
 {
-	const int	h = (threadIdx.x & 63) >> 5;
-	const uint32_t r0 = rb * 32 + 4 * h;
-
-	if (q >= o.nq || rb * 32 >= o.n)
-		return;
-	T		   *out = (T *) o.out + (int64_t) q * o.ostride;
+	const int	lane = threadIdx.x & 63;
+	const uint32_t r = rb * 32 + (lane & 31), qh = q0 + 4 * (lane >> 5);
+	T		   *out = (T *) o.out + (int64_t) qh * o.ostride + r;
+	float		s[16];
 
 #pragma unroll
 	for (int g4 = 0; g4 < 4; g4++)
 	{
-		const uint32_t r = r0 + 8 * g4;
-		const float4 r4 = *(const float4 *) (rs + 8 * g4 + 4 * h);
-		float		s[4] = {i8_score(acc[4 * g4], r4.x, qs), i8_score(acc[4 * g4 + 1], r4.y, qs),
-			i8_score(acc[4 * g4 + 2], r4.z, qs), i8_score(acc[4 * g4 + 3], r4.w, qs)};
-		const float4 b4 = BIAS ? *(const float4 *) (bias + 8 * g4 + 4 * h) : make_float4(0, 0, 0, 0);
-		I8Vec<T, 4> v;
+		const float4 q4 = *(const float4 *) (qs + 8 * g4 + 4 * (lane >> 5));
+		const float qv[4] = {q4.x, q4.y, q4.z, q4.w};
 
 #pragma unroll
 		for (int j = 0; j < 4; j++)
 		{
+			s[4 * g4 + j] = i8_score(acc[4 * g4 + j], rs, qv[j]);
 			if (BIAS)
-				s[j] = s[j] + (&b4.x)[j];
-			v.v[j] = I8Elem<T>::store(s[j]);
+				s[4 * g4 + j] = s[4 * g4 + j] + bias;
 		}
-		if (o.ovec && r + 4 <= o.n)
-			*(I8Vec<T, 4> *) (out + r) = v;
-		else
-#pragma unroll
-			for (int j = 0; j < 4; j++)
-				if (r + j < o.n)
-					out[r + j] = v.v[j];
 	}
+	if (r >= o.n)
+		return;
+	if (q0 + 32 <= o.nq)
+#pragma unroll
+		for (int i = 0; i < 16; i++)
+			out[(int64_t) (8 * (i / 4) + i % 4) * o.ostride] = I8Elem<T>::store(s[i]);
+	else
+#pragma unroll
+		for (int i = 0; i < 16; i++)
+			if (qh + 8 * (i / 4) + i % 4 < o.nq)
+				out[(int64_t) (8 * (i / 4) + i % 4) * o.ostride] = I8Elem<T>::store(s[i]);
 }
 
 /*
- * The largest score that takes part among the 32 rows of block rb, for the lane's query (both halves of the wave hold it).
+ * The largest score that takes part among the 32 rows of a block, for the lane's query (both halves of the wave hold it).
+ * The rows were the matrix instruction's first operand: lane l has query l % 32 and, in register 4 g + j, row 8 g + 4 (l / 32) + j.
  * rs, bias: the block's 32 row scales and biases (in LDS).  fmaxf drops NaN: rows of NaN scores, padding rows among them, never take
  * part.  A product with a positive finite query scale rises with its other factor and so does its rounding, hence without
  * a bias RN(t * qs) is taken of the largest t only.
@@ -460,7 +460,7 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 {
 	constexpr int U = TB == 1 ? 8 : 4;
 	__shared__ __attribute__((aligned(16))) float s_m[KIND::MODE == 1 ? TB * 32 : 1][4];
-	__shared__ __attribute__((aligned(16))) float s_rs[4][32], s_bias[KIND::BIAS ? 4 : 1][32];
+	__shared__ __attribute__((aligned(16))) float s_rs[4][32], s_bias[KIND::BIAS ? 4 : 1][32], s_qs[4][KIND::MODE == 0 ? TB * 32 : 1];
 	const int	lane = threadIdx.x & 63;
 	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const uint32_t rb = min(blockIdx.x * 4 + wave, nrb - 1);	/* (waves behind the last block do it over) */
@@ -503,7 +503,8 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 			if (k + u * 32 < kp)
 #pragma unroll
 				for (int t = 0; t < TB; t++)
-					acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[u], bv[u][t], acc[t], 0, 0, 0);
+					acc[t] = KIND::MODE == 0 ? __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[u][t], av[u], acc[t], 0, 0, 0) :
+						__builtin_amdgcn_mfma_i32_32x32x32_i8(av[u], bv[u][t], acc[t], 0, 0, 0);
 	}
 	/* (a wave's own LDS: what it writes it reads in order) */
 	if (lane < 32)
@@ -511,15 +512,17 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 		s_rs[wave][lane] = my_rs;
 		if (KIND::BIAS)
 			s_bias[wave][lane] = my_bias;
+		if (KIND::MODE == 0)
+#pragma unroll
+			for (int t = 0; t < TB; t++)
+				s_qs[wave][t * 32 + lane] = qs[t];
 	}
 	__builtin_amdgcn_wave_barrier();
 #pragma unroll
 	for (int t = 0; t < TB; t++)
 	{
-		const uint32_t q = (qb0 + t) * 32 + (lane & 31);
-
 		if (KIND::MODE == 0)
-			i8_write_scores<KIND::BIAS, typename KIND::T>(o, s_rs[wave], s_bias[KIND::BIAS ? wave : 0], rb, q, qs[t], acc[t]);
+			i8_write_scores<KIND::BIAS, typename KIND::T>(o, my_rs, my_bias, s_qs[wave] + t * 32, rb, (qb0 + t) * 32, acc[t]);
 		else
 		{
 			const float m = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs[wave], s_bias[KIND::BIAS ? wave : 0], bits[t], qs[t], acc[t]);
@@ -720,6 +723,10 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 	read(0, 0);
 
 	uint32_t	buf = 0, slot = 0;
+	auto		mul = [](const i8_v4i &r, const i8_v4i &q, const i8_v16i &c) -> i8_v16i {
+		return KIND::MODE == 0 ? __builtin_amdgcn_mfma_i32_32x32x32_i8(q, r, c, 0, 0, 0) :
+			__builtin_amdgcn_mfma_i32_32x32x32_i8(r, q, c, 0, 0, 0);
+	};
 
 	/*
 	 * A stage, its first half's operands in registers.  FIRST: the tile's first stage, sums start from zero.  The next stage
@@ -736,7 +743,7 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 		for (int i = 0; i < 4; i++)
 #pragma unroll
 			for (int t = 0; t < WQ; t++)
-				acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[0][i], bv[0][t], FIRST ? zero : acc[i][t], 0, 0, 0);
+				acc[i][t] = mul(av[0][i], bv[0][t], FIRST ? zero : acc[i][t]);
 		__builtin_amdgcn_sched_barrier(0);
 		i8_wait_vm<(I8_NBUF - 2) * PER>();
 		asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -750,7 +757,7 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 #pragma unroll
 			for (int t = 0; t < WQ; t++)
 			{
-				acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[1][i], bv[1][t], acc[i][t], 0, 0, 0);
+				acc[i][t] = mul(av[1][i], bv[1][t], acc[i][t]);
 				if (i * WQ + t < PER)
 					c_copy(i * WQ + t);
 				__builtin_amdgcn_sched_barrier(0);
@@ -769,18 +776,18 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 #pragma unroll
 		for (int t = 0; t < WQ; t++)
 		{
-			const uint32_t q = (qb0 + t) * 32 + (lane & 31);
-			const float qs = s_qs[slot][(wq * WQ + t) * 32 + (lane & 31)];
-
 			if (KIND::MODE == 0)
 			{
 #pragma unroll
 				for (int i = 0; i < 4; i++)
-					i8_write_scores<KIND::BIAS, typename KIND::T>(o, s_rs[slot] + (wr * 4 + i) * 32,
-																  s_bias[KIND::BIAS ? slot : 0] + (wr * 4 + i) * 32, rb0 + i, q, qs, acc[i][t]);
+					i8_write_scores<KIND::BIAS, typename KIND::T>(o, s_rs[slot][(wr * 4 + i) * 32 + (lane & 31)],
+																  s_bias[KIND::BIAS ? slot : 0][(wr * 4 + i) * 32 + (lane & 31)],
+																  s_qs[slot] + (wq * WQ + t) * 32, rb0 + i, (qb0 + t) * 32, acc[i][t]);
 			}
 			else
 			{
+				const uint32_t q = (qb0 + t) * 32 + (lane & 31);
+				const float qs = s_qs[slot][(wq * WQ + t) * 32 + (lane & 31)];
 				float		m[4];
 
 #pragma unroll
@@ -1052,27 +1059,34 @@ i8_rescore(const unsigned char *rows, const unsigned char *queries, uint32_t kp,
 	const unsigned char *a = rows + (size_t) rb * 32u * kp + lane * 16;
 	const unsigned char *b = queries + (size_t) (q >> 5) * 32u * kp + (q & 31) * 16 + (lane >> 5) * 512;
 	const uint32_t r = rb * 32 + (lane & 31);
+	const float rs = o.rscale[r], qs = o.qscale[q], bias = o.bias && r < o.n ? o.bias[r] : 0.0f;
+	const uint32_t bits = o.mask ? o.mask[(int64_t) q * o.mask_stride + rb] : 0xFFFFFFFFu;
 	int			s = 0;
 
-#pragma unroll 8
-	for (uint32_t e = 0; e < kp; e += 32)
+	for (uint32_t e = 0; e < kp; e += 256)
 	{
-		const i8_v4i x = *(const i8_v4i *) (a + (size_t) e * 32);
-		const i8_v4i y = *(const i8_v4i *) (b + (size_t) e * 32);
+		i8_v4i		x[8], y[8];
 
 #pragma unroll
-		for (int i = 0; i < 4; i++)
-			s = __builtin_amdgcn_sdot4(x[i], y[i], s, false);
+		for (int u = 0; u < 8; u++)
+		{
+			x[u] = *(const i8_v4i *) (a + (size_t) min(e + u * 32, kp - 32) * 32);
+			y[u] = *(const i8_v4i *) (b + (size_t) min(e + u * 32, kp - 32) * 32);
+		}
+#pragma unroll
+		for (int u = 0; u < 8; u++)
+			if (e + u * 32 < kp)
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					s = __builtin_amdgcn_sdot4(x[u][i], y[u][i], s, false);
 	}
 	s += __shfl_xor(s, 32, 64);
 
-	float		v = i8_score(s, o.rscale[r], o.qscale[q]);
+	float		v = i8_score(s, rs, qs);
 
-	if (o.bias && r < o.n)
-		v = v + o.bias[r];
-	if (!(v > I8_NINF) || (o.mask && !(o.mask[(int64_t) q * o.mask_stride + rb] >> (lane & 31) & 1u)))
-		v = I8_NINF;
-	return v;
+	if (o.bias)
+		v = v + bias;
+	return v > I8_NINF && (bits >> (lane & 31) & 1u) ? v : I8_NINF;
 }
 
 template <int NT>
@@ -1845,7 +1859,6 @@ ndbhip_i8_product_device(const ndbhip_i8 *t, const void *d_q, int q_type, const 
 		o.bias = d_bias;
 		o.out = (char *) d_out + q0 * out_stride * osz;
 		o.ostride = out_stride;
-		o.ovec = i8_aligned(d_out, out_stride * osz, 4 * osz);
 		o.n = (uint32_t) t->n;
 		o.nq = (uint32_t) m;
 		const unsigned char *qc = (const unsigned char *) d_ws + w.q_off;

@@ -8,6 +8,7 @@ and can be captured into a graph (the workspace of a call comes from torch's all
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import numpy as np
 
@@ -21,44 +22,66 @@ def _bad(msg):
     return NdbHipError(ERR_INVALID, msg)
 
 
-def _types():
-    import torch
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+class _Torch:
+    """torch and what is asked of it at every call, looked up once (the package itself loads without torch)"""
 
-
-class _OnTorchStream:
-    """The library's work of this thread on torch's current stream of the library's device, for the calls inside."""
-
-    def __enter__(self):
+    def __init__(self):
         import torch
-        s = torch.cuda.current_stream(_lib._device).cuda_stream
-        self.prev = C.c_void_p()
-        check(lib().ndbhip_swap_thread_stream(C.c_void_p(s or STREAM_LEGACY), C.byref(self.prev)))
-        return self
-
-    def __exit__(self, *exc):
-        check(lib().ndbhip_swap_thread_stream(self.prev, C.byref(C.c_void_p())))
-        return False
-
-
-def _here():
-    """the library's device, initialised on torch's current one if it is not yet"""
-    import torch
-    if not _lib._inited:
-        ensure_init(torch.cuda.current_device())
-    return torch.device("cuda", _lib._device)
+        if not _lib._inited:
+            ensure_init(torch.cuda.current_device())
+        self.torch = torch
+        self.types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+        self.floats = (torch.float32, torch.float16, torch.bfloat16)
+        self.f32, self.i8, self.i32, self.i64 = (torch.float32,), (torch.int8,), (torch.int32,), (torch.int64,)
+        self.words = (torch.int32, torch.uint32) if hasattr(torch, "uint32") else (torch.int32,)
+        self.device = torch.device("cuda", _lib._device)
+        self.lib = lib()
 
 
-def _tensor(t, name, dtypes, ndim, device):
-    """checks what every tensor argument has to be; the last dimension's elements are neighbours"""
-    import torch
-    if not isinstance(t, torch.Tensor):
+_state = None
+
+
+def _torch():
+    global _state
+    if _state is None:
+        _state = _Torch()
+    return _state
+
+
+class _Previous(threading.local):
+    def __init__(self):
+        self.p = C.c_void_p()
+        self.ref = C.byref(self.p)
+
+
+_previous = _Previous()
+
+
+def _call(fn, *args):
+    """One call of the library on torch's current stream of the library's device; the thread's stream is as before afterwards."""
+    T = _state
+    swap = T.lib.ndbhip_swap_thread_stream
+    ref = _previous.ref
+    check(swap(T.torch.cuda.current_stream(T.device).cuda_stream or STREAM_LEGACY, ref))
+    prev = _previous.p.value
+    try:
+        rc = fn(*args)
+        if rc:
+            raise NdbHipError(rc, _lib.last_error())
+    finally:
+        swap(prev, ref)
+
+
+def _tensor(t, name, dtypes, ndim):
+    """checks what every tensor argument has to be"""
+    T = _state
+    if not isinstance(t, T.torch.Tensor):
         raise _bad(f"{name} must be a torch tensor")
-    if t.device != device:
-        raise _bad(f"{name} is on {t.device}, the library on {device}")
+    if t.device != T.device:
+        raise _bad(f"{name} is on {t.device}, the library on {T.device}")
     if t.dtype not in dtypes:
         raise _bad(f"{name} must be one of {[str(d) for d in dtypes]}, not {t.dtype}")
-    if t.dim() not in (ndim if isinstance(ndim, tuple) else (ndim,)):
+    if t.dim() != ndim and (type(ndim) is int or t.dim() not in ndim):
         raise _bad(f"{name} has {t.dim()} dimensions")
     return t
 
@@ -77,59 +100,51 @@ def _out_rows(t, name):
 
 
 def _p(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
-
-
-def _floats():
-    import torch
-    return (torch.float32, torch.float16, torch.bfloat16)
+    return None if t is None else t.data_ptr()
 
 
 def quantize_rows(x, codes=None, scales=None):
     """Rows [n, dim] (float32, float16, bfloat16) -> (codes int8 [n, dim], scales float32 [n]); ndbhip_i8_quantize_device."""
-    import torch
-    dev = _here()
-    x, stride = _rows(_tensor(x, "x", _floats(), 2, dev))
+    T = _torch()
+    x, stride = _rows(_tensor(x, "x", T.floats, 2))
     n, dim = x.shape
     if codes is None:
-        codes = torch.empty((n, dim), dtype=torch.int8, device=dev)
+        codes = T.torch.empty((n, dim), dtype=T.torch.int8, device=T.device)
+        cstride = dim
+    else:
+        cstride = _out_rows(_tensor(codes, "codes", T.i8, 2), "codes")
     if scales is None:
-        scales = torch.empty(n, dtype=torch.float32, device=dev)
-    _tensor(codes, "codes", (torch.int8,), 2, dev)
-    _tensor(scales, "scales", (torch.float32,), 1, dev)
-    if codes.shape != x.shape or scales.shape != (n,) or not scales.is_contiguous():
+        scales = T.torch.empty(n, dtype=T.torch.float32, device=T.device)
+    else:
+        _tensor(scales, "scales", T.f32, 1)
+    if codes.shape != x.shape or scales.shape[0] != n or not scales.is_contiguous():
         raise _bad("codes must be [n, dim] and scales [n], contiguous")
-    with _OnTorchStream():
-        check(lib().ndbhip_i8_quantize_device(_p(x), _types()[x.dtype], n, dim, stride, _p(codes), _out_rows(codes, "codes"), _p(scales)))
+    _call(T.lib.ndbhip_i8_quantize_device, _p(x), T.types[x.dtype], n, dim, stride, _p(codes), cstride, _p(scales))
     return codes, scales
 
 
 def dequantize_rows(codes, scales, dtype=None, out=None):
     """The values (codes int8 [n, dim], scales float32 [n]) stand for, as float32 (or `dtype`); ndbhip_i8_dequantize_device."""
-    import torch
-    dev = _here()
-    codes, stride = _rows(_tensor(codes, "codes", (torch.int8,), 2, dev))
-    scales = _tensor(scales, "scales", (torch.float32,), 1, dev).contiguous()
-    if scales.shape[0] != codes.shape[0]:
+    T = _torch()
+    codes, stride = _rows(_tensor(codes, "codes", T.i8, 2))
+    scales = _tensor(scales, "scales", T.f32, 1).contiguous()
+    n, dim = codes.shape
+    if scales.shape[0] != n:
         raise _bad("a scale for every row")
     if out is None:
-        out = torch.empty(codes.shape, dtype=dtype or torch.float32, device=dev)
-    _tensor(out, "out", _floats(), 2, dev)
+        out = T.torch.empty((n, dim), dtype=dtype or T.torch.float32, device=T.device)
+    _tensor(out, "out", T.floats, 2)
     if out.shape != codes.shape or dtype not in (None, out.dtype):
         raise _bad("out must have the codes' shape and the dtype asked for")
-    with _OnTorchStream():
-        check(lib().ndbhip_i8_dequantize_device(_p(codes), stride, _p(scales), codes.shape[0], codes.shape[1], _p(out),
-                                                _types()[out.dtype], _out_rows(out, "out")))
+    _call(T.lib.ndbhip_i8_dequantize_device, _p(codes), stride, _p(scales), n, dim, _p(out), T.types[out.dtype], _out_rows(out, "out"))
     return out
 
 
-def _mask_arg(mask, nq, n, dev):
+def _mask_arg(mask, nq, n):
     """(tensor, words from one query's mask to the next)"""
-    import torch
     if mask is None:
         return None, 0
-    words = {torch.int32} | ({torch.uint32} if hasattr(torch, "uint32") else set())
-    _tensor(mask, "mask", tuple(words), (1, 2), dev)
+    _tensor(mask, "mask", _state.words, (1, 2))
     m = mask[None] if mask.dim() == 1 else mask
     if m.shape[0] not in (1, nq) or m.shape[1] < (n + 31) // 32:
         raise _bad(f"mask must be [words] or [1 or {nq}, words] with at least {(n + 31) // 32} words of 32 rows")
@@ -137,11 +152,10 @@ def _mask_arg(mask, nq, n, dev):
     return m, 0 if m.shape[0] == 1 else stride
 
 
-def _bias_arg(bias, nq, n, dev, per_query):
-    import torch
+def _bias_arg(bias, nq, n, per_query):
     if bias is None:
         return None, 0
-    _tensor(bias, "bias", (torch.float32,), (1, 2) if per_query else 1, dev)
+    _tensor(bias, "bias", _state.f32, (1, 2) if per_query else 1)
     b = bias[None] if bias.dim() == 1 else bias
     if b.shape[0] not in (1, nq) or b.shape[1] != n:
         raise _bad(f"bias must be [{n}]" + (f" or [1 or {nq}, {n}]" if per_query else ""))
@@ -158,36 +172,34 @@ def adjust_scores(scores, seen=None, penalties=None, bias=None, mask=None, out=N
     mask       int32 words [ceil(n / 32)] or [nq, ceil(n / 32)], bit i % 32 of word i / 32: 0 = -inf
     out        another tensor of the scores' shape and type, or `scores` itself (in place); None: a new one
     """
-    import torch
-    dev = _here()
-    _tensor(scores, "scores", _floats(), 2, dev)
+    T = _torch()
+    _tensor(scores, "scores", T.floats, 2)
     nq, n = scores.shape
     if out is not None:
-        _tensor(out, "out", (scores.dtype,), 2, dev)
+        _tensor(out, "out", (scores.dtype,), 2)
         if out.shape != scores.shape:
             raise _bad("out must have the scores' shape")
         ostride = _out_rows(out, "out")
     src, stride = _rows(scores)
     if out is None:
-        out = torch.empty((nq, n), dtype=scores.dtype, device=dev)
+        out = T.torch.empty((nq, n), dtype=scores.dtype, device=T.device)
         ostride = n
     off = ids = None
     if (seen is None) != (penalties is None):
         raise _bad("seen and penalties go together")
     if seen is not None:
         off, ids = seen
-        off = _tensor(off, "offsets", (torch.int64,), 1, dev).contiguous()
-        ids = _tensor(ids, "ids", (torch.int32,), 1, dev).contiguous()
-        penalties = _tensor(penalties, "penalties", (torch.float32,), 2, dev).contiguous()
+        off = _tensor(off, "offsets", T.i64, 1).contiguous()
+        ids = _tensor(ids, "ids", T.i32, 1).contiguous()
+        penalties = _tensor(penalties, "penalties", T.f32, 2).contiguous()
         if off.shape[0] != nq + 1 or penalties.shape != (nq, 3):
             raise _bad("offsets must be [nq + 1] and penalties [nq, 3]")
         if ids.numel() == 0:
             off = ids = penalties = None
-    bias, bstride = _bias_arg(bias, nq, n, dev, True)
-    mask, mstride = _mask_arg(mask, nq, n, dev)
-    with _OnTorchStream():
-        check(lib().ndbhip_scores_adjust_device(_p(src), _types()[src.dtype], nq, n, stride, _p(off), _p(ids), _p(penalties), _p(bias),
-                                                bstride, _p(mask), mstride, _p(out), ostride))
+    bias, bstride = _bias_arg(bias, nq, n, True)
+    mask, mstride = _mask_arg(mask, nq, n)
+    _call(T.lib.ndbhip_scores_adjust_device, _p(src), T.types[src.dtype], nq, n, stride, _p(off), _p(ids), _p(penalties), _p(bias), bstride,
+          _p(mask), mstride, _p(out), ostride)
     return out
 
 
@@ -203,6 +215,8 @@ class Int8Table:
         h = C.c_void_p()
         check(lib().ndbhip_i8_create(self.dim, C.byref(h)))
         self._h = h
+        self._n = 0
+        self._ws = {}            # (queries, k) -> bytes of workspace, for the rows there are
 
     def close(self):
         if getattr(self, "_h", None):
@@ -217,105 +231,109 @@ class Int8Table:
 
     @property
     def nrows(self) -> int:
-        return int(lib().ndbhip_i8_nrows(self._h))
+        return self._n
+
+    def _loaded(self):
+        self._n = int(lib().ndbhip_i8_nrows(self._h))
+        self._ws.clear()
 
     def load(self, rows, scales=None):
         """The table's rows, in place of what it held: a numpy float32 array or a tensor [n, dim] of float32, float16,
         bfloat16 — quantised on the way — or of int8 with their scales [n]."""
-        import torch
         if isinstance(rows, np.ndarray):
             if scales is not None:
                 raise _bad("scales go with int8 tensors")
             r = np.ascontiguousarray(rows, dtype=np.float32)
             if r.ndim != 2 or r.shape[1] != self.dim:
                 raise _bad(f"rows must be [n, {self.dim}]")
-            check(lib().ndbhip_i8_load(self._h, r.ctypes.data_as(C.c_void_p), r.shape[0]))
+            try:
+                check(lib().ndbhip_i8_load(self._h, r.ctypes.data, r.shape[0]))
+            finally:
+                self._loaded()
             return
-        dev = _here()
-        r, stride = _rows(_tensor(rows, "rows", tuple(_types()), 2, dev))
+        T = _torch()
+        r, stride = _rows(_tensor(rows, "rows", tuple(T.types), 2))
         if r.shape[1] != self.dim:
             raise _bad(f"rows must be [n, {self.dim}]")
-        if (r.dtype == torch.int8) != (scales is not None):
+        if (r.dtype == T.torch.int8) != (scales is not None):
             raise _bad("scales go with int8 rows, and only with them")
         if scales is not None:
-            scales = _tensor(scales, "scales", (torch.float32,), 1, dev).contiguous()
+            scales = _tensor(scales, "scales", T.f32, 1).contiguous()
             if scales.shape[0] != r.shape[0]:
                 raise _bad("a scale for every row")
-        with _OnTorchStream():
-            check(lib().ndbhip_i8_load_device(self._h, _p(r), _types()[r.dtype], r.shape[0], stride, _p(scales)))
+        try:
+            _call(T.lib.ndbhip_i8_load_device, self._h, _p(r), T.types[r.dtype], r.shape[0], stride, _p(scales))
+        finally:
+            self._loaded()
 
     def export(self):
         """(codes int8 [n, dim], scales float32 [n])"""
-        import torch
-        dev = _here()
-        n = self.nrows
-        codes = torch.empty((n, self.dim), dtype=torch.int8, device=dev)
-        scales = torch.empty(n, dtype=torch.float32, device=dev)
-        with _OnTorchStream():
-            check(lib().ndbhip_i8_export_device(self._h, _p(codes), self.dim, _p(scales)))
+        T = _torch()
+        codes = T.torch.empty((self._n, self.dim), dtype=T.torch.int8, device=T.device)
+        scales = T.torch.empty(self._n, dtype=T.torch.float32, device=T.device)
+        _call(T.lib.ndbhip_i8_export_device, self._h, _p(codes), self.dim, _p(scales))
         return codes, scales
 
-    def _queries(self, queries, dev):
-        import torch
+    def _queries(self, queries):
+        T = _torch()
         scales = None
         if isinstance(queries, (tuple, list)):
             queries, scales = queries
-            scales = _tensor(scales, "query scales", (torch.float32,), 1, dev).contiguous()
-        q, stride = _rows(_tensor(queries, "queries", tuple(_types()), 2, dev))
+            scales = _tensor(scales, "query scales", T.f32, 1).contiguous()
+        q, stride = _rows(_tensor(queries, "queries", T.types, 2))
         if q.shape[1] != self.dim:
             raise _bad(f"queries must be [nq, {self.dim}]")
-        if (q.dtype == torch.int8) != (scales is not None) or scales is not None and scales.shape[0] != q.shape[0]:
+        if (q.dtype == T.torch.int8) != (scales is not None) or scales is not None and scales.shape[0] != q.shape[0]:
             raise _bad("int8 queries come as (codes [nq, dim], scales [nq]), others alone")
-        return q, stride, scales
+        return T, q, stride, scales
 
-    def _workspace(self, nq, k, dev):
-        import torch
-        b = C.c_size_t(0)
-        check(lib().ndbhip_i8_workspace(self._h, nq, k, C.byref(b)))
-        return torch.empty(max(b.value, 1), dtype=torch.uint8, device=dev), b.value
+    def _workspace(self, T, nq, k):
+        b = self._ws.get((nq, k))
+        if b is None:
+            if len(self._ws) >= 4096:
+                self._ws.clear()
+            out = C.c_size_t(0)
+            check(lib().ndbhip_i8_workspace(self._h, nq, k, C.byref(out)))
+            b = self._ws[(nq, k)] = out.value
+        return T.torch.empty(b, dtype=T.torch.uint8, device=T.device), b
 
     def scores(self, queries, bias=None, dtype=None, out=None):
         """Every score: [nq, nrows] of float32 (or `dtype`, or into `out`); ndbhip_i8_product_device.  queries: [nq, dim] of
         float32, float16, bfloat16, or (codes, scales)."""
-        import torch
-        dev = _here()
-        q, stride, qs = self._queries(queries, dev)
-        nq, n = q.shape[0], self.nrows
-        bias, _ = _bias_arg(bias, 1, n, dev, False)
+        T, q, stride, qs = self._queries(queries)
+        nq, n = q.shape[0], self._n
+        bias, _ = _bias_arg(bias, 1, n, False)
         if out is None:
-            out = torch.empty((nq, n), dtype=dtype or torch.float32, device=dev)
-        _tensor(out, "out", _floats(), 2, dev)
+            out = T.torch.empty((nq, n), dtype=dtype or T.torch.float32, device=T.device)
+        _tensor(out, "out", T.floats, 2)
         if out.shape != (nq, n) or dtype not in (None, out.dtype):
             raise _bad(f"out must be [{nq}, {n}] and of the dtype asked for")
-        ws, wsb = self._workspace(nq, 0, dev)
-        with _OnTorchStream():
-            check(lib().ndbhip_i8_product_device(self._h, _p(q), _types()[q.dtype], _p(qs), nq, stride, _p(bias), _p(out),
-                                                 _types()[out.dtype], _out_rows(out, "out"), _p(ws), wsb))
+        ostride = _out_rows(out, "out")
+        ws, wsb = self._workspace(T, nq, 0)
+        _call(T.lib.ndbhip_i8_product_device, self._h, _p(q), T.types[q.dtype], _p(qs), nq, stride, _p(bias), _p(out), T.types[out.dtype],
+              ostride, _p(ws), wsb)
         return out
 
     def search(self, queries, k, bias=None, mask=None):
         """The k best rows of each query: (ids int64 [nq, k], scores float32 [nq, k]), higher scores first, equal ones by id; places
         no row fills hold -1 and -inf.  ndbhip_i8_search_device.  bias: float32 [nrows]; mask: as in adjust_scores.  numpy float32
         queries (and numpy bias, mask uint32 / int32) take the host form and return numpy arrays."""
-        import torch
         if isinstance(queries, np.ndarray):
             return self._search_host(queries, int(k), bias, mask)
-        dev = _here()
-        q, stride, qs = self._queries(queries, dev)
-        nq, n, k = q.shape[0], self.nrows, int(k)
-        bias, _ = _bias_arg(bias, 1, n, dev, False)
-        mask, mstride = _mask_arg(mask, nq, n, dev)
-        ws, wsb = self._workspace(nq, k, dev)
-        ids = torch.empty((nq, max(k, 0)), dtype=torch.int64, device=dev)
-        scores = torch.empty((nq, max(k, 0)), dtype=torch.float32, device=dev)
-        with _OnTorchStream():
-            check(lib().ndbhip_i8_search_device(self._h, _p(q), _types()[q.dtype], _p(qs), nq, stride, _p(bias), _p(mask), mstride, k,
-                                                _p(ids), _p(scores), _p(ws), wsb))
+        T, q, stride, qs = self._queries(queries)
+        nq, n, k = q.shape[0], self._n, int(k)
+        bias, _ = _bias_arg(bias, 1, n, False)
+        mask, mstride = _mask_arg(mask, nq, n)
+        ws, wsb = self._workspace(T, nq, k)
+        ids = T.torch.empty((nq, k), dtype=T.torch.int64, device=T.device)
+        scores = T.torch.empty((nq, k), dtype=T.torch.float32, device=T.device)
+        _call(T.lib.ndbhip_i8_search_device, self._h, _p(q), T.types[q.dtype], _p(qs), nq, stride, _p(bias), _p(mask), mstride, k, _p(ids),
+              _p(scores), _p(ws), wsb)
         return ids, scores
 
     def _search_host(self, queries, k, bias, mask):
         q = np.ascontiguousarray(queries, dtype=np.float32)
-        n = self.nrows
+        n = self._n
         if q.ndim != 2 or q.shape[1] != self.dim:
             raise _bad(f"queries must be [nq, {self.dim}]")
         p = lambda a: None if a is None else a.ctypes.data_as(C.c_void_p)     # noqa: E731
