@@ -978,7 +978,7 @@ i8_pick(I8Select<NT, CAP> &S, uint32_t *quads, const float *gm, const float *qm,
 {
 	const uint32_t nquad = (ng + 3) / 4;
 	float		t = I8_NINF;
-	uint32_t	groups = NT / 64;
+	uint32_t	groups = max(NT / 64, 16);
 
 	while (groups < 2 * k && groups < NT)
 		groups <<= 1;
@@ -1007,14 +1007,17 @@ i8_pick(I8Select<NT, CAP> &S, uint32_t *quads, const float *gm, const float *qm,
 			const float mine = S.top[threadIdx.x];
 			uint32_t	r = 0;
 
-			for (uint32_t j = 0; j < groups; j += 8)
-#pragma unroll
-				for (uint32_t e = 0; e < 8; e++)
-				{
-					const float o = S.top[j + e];
+			for (uint32_t j = 0; j < groups; j += 16)	/* (groups: at least 16; sixteen reads in flight, no branches) */
+			{
+				float		o[16];
 
-					r += o > mine || (o == mine && j + e < threadIdx.x) ? 1u : 0u;
-				}
+#pragma unroll
+				for (uint32_t e = 0; e < 16; e++)
+					o[e] = S.top[j + e];
+#pragma unroll
+				for (uint32_t e = 0; e < 16; e++)
+					r += (uint32_t) (o[e] > mine) | ((uint32_t) (o[e] == mine) & (uint32_t) (j + e < threadIdx.x));
+			}
 			if (r == k - 1)
 				S.floor = mine;
 		}
@@ -1050,43 +1053,64 @@ i8_pick(I8Select<NT, CAP> &S, uint32_t *quads, const float *gm, const float *qm,
 	}, nq4 * 4, k, floor2);
 }
 
-/* the scores of the 32 rows of block rb for query q, one a lane in both halves of the wave: a lane sums 16-byte pieces of
- * row l % 32 against the query's, the halves joined at the end; rows that take no part: -inf */
-__device__ __forceinline__ float
-i8_rescore(const unsigned char *rows, const unsigned char *queries, uint32_t kp, const I8Out &o, uint32_t rb, uint32_t q)
+/*
+ * Scoring picked blocks again.  A wave takes a part, up to 8 steps of 32 dimensions, of one block and asks for all of it at
+ * once: the rows are anywhere in the table, so what counts is how many requests are under way.  A lane sums 16-byte pieces
+ * of row l % 32 against the query's, the two halves of the wave are joined, and the parts of a block add up in LDS.
+ */
+#define I8_PART 8u
+__device__ __forceinline__ int
+i8_part_sum(const unsigned char *rows, const unsigned char *queries, uint32_t kp, uint32_t rb, uint32_t q, uint32_t part)
 {
 	const int	lane = threadIdx.x & 63;
+	const uint32_t e0 = part * I8_PART * 32;
 	const unsigned char *a = rows + (size_t) rb * 32u * kp + lane * 16;
 	const unsigned char *b = queries + (size_t) (q >> 5) * 32u * kp + (q & 31) * 16 + (lane >> 5) * 512;
-	const uint32_t r = rb * 32 + (lane & 31);
-	const float rs = o.rscale[r], qs = o.qscale[q], bias = o.bias && r < o.n ? o.bias[r] : 0.0f;
-	const uint32_t bits = o.mask ? o.mask[(int64_t) q * o.mask_stride + rb] : 0xFFFFFFFFu;
+	i8_v4i		x[I8_PART], y[I8_PART];
 	int			s = 0;
 
-	for (uint32_t e = 0; e < kp; e += 256)
-	{
-		i8_v4i		x[8], y[8];
-
 #pragma unroll
-		for (int u = 0; u < 8; u++)
+	for (uint32_t u = 0; u < I8_PART; u++)
+		if (e0 + u * 32 < kp)
 		{
-			x[u] = *(const i8_v4i *) (a + (size_t) min(e + u * 32, kp - 32) * 32);
-			y[u] = *(const i8_v4i *) (b + (size_t) min(e + u * 32, kp - 32) * 32);
+			x[u] = *(const i8_v4i *) (a + (size_t) (e0 + u * 32) * 32);
+			y[u] = *(const i8_v4i *) (b + (size_t) (e0 + u * 32) * 32);
 		}
 #pragma unroll
-		for (int u = 0; u < 8; u++)
-			if (e + u * 32 < kp)
+	for (uint32_t u = 0; u < I8_PART; u++)
+		if (e0 + u * 32 < kp)
 #pragma unroll
-				for (int i = 0; i < 4; i++)
-					s = __builtin_amdgcn_sdot4(x[u][i], y[u][i], s, false);
-	}
-	s += __shfl_xor(s, 32, 64);
+			for (int i = 0; i < 4; i++)
+				s = __builtin_amdgcn_sdot4(x[u][i], y[u][i], s, false);
+	return s + __shfl_xor(s, 32, 64);
+}
 
-	float		v = i8_score(s, rs, qs);
+/* what the sums of row i of block rb become a score with */
+struct I8Row
+{
+	float		rs, bias;
+	uint32_t	bits;
+};
+__device__ __forceinline__ I8Row
+i8_row(const I8Out &o, uint32_t rb, uint32_t i, uint32_t q)
+{
+	const uint32_t r = rb * 32 + i;
+	I8Row		w;
+
+	w.rs = o.rscale[r];
+	w.bias = o.bias && r < o.n ? o.bias[r] : 0.0f;
+	w.bits = o.mask ? o.mask[(int64_t) q * o.mask_stride + rb] >> i : 1u;
+	return w;
+}
+/* -inf for rows that take no part */
+__device__ __forceinline__ float
+i8_row_score(const I8Out &o, const I8Row &w, int dot, float qs)
+{
+	float		v = i8_score(dot, w.rs, qs);
 
 	if (o.bias)
-		v = v + bias;
-	return v > I8_NINF && (bits >> (lane & 31) & 1u) ? v : I8_NINF;
+		v = v + w.bias;
+	return v > I8_NINF && (w.bits & 1u) ? v : I8_NINF;
 }
 
 template <int NT>
@@ -1114,24 +1138,36 @@ k_i8_finish(const unsigned char *__restrict__ rows, const unsigned char *__restr
 {
 	__shared__ I8Select<NT, 512> S;
 	__shared__ uint32_t picked[I8_FUSED_K];
-	__shared__ float cand[I8_FUSED_K * 32];
+	__shared__ int sum[I8_FUSED_K * 32];		/* (a score's bits take the place of its sum) */
 	const uint32_t q = blockIdx.x;
+	const float qs = o.qscale[q];
 	const uint32_t kk = i8_pick(S, picked, o.gmax + (size_t) q * o.ngp, o.qmax + (size_t) q * (o.ngp / 4), (o.n + 31) / 32, k);
 	const float floor = kk == k ? i8_word_score(S.list[k - 1]) : I8_NINF;
+	const uint32_t parts = (kp + 32 * I8_PART - 1) / (32 * I8_PART);
 
 	for (uint32_t i = threadIdx.x; i < kk; i += NT)
 		picked[i] = (uint32_t) S.list[i];
+	for (uint32_t i = threadIdx.x; i < kk * 32; i += NT)
+		sum[i] = 0;
 	__syncthreads();
-	for (uint32_t slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); slot < kk; slot += NT / 64)
+	I8Row		first = {};
+
+	if (threadIdx.x < kk * 32)
+		first = i8_row(o, picked[threadIdx.x / 32], threadIdx.x % 32, q);
+	for (uint32_t item = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); item < kk * parts; item += NT / 64)
 	{
-		const float v = i8_rescore(rows, queries, kp, o, picked[slot], q);
+		const uint32_t slot = item / parts;
+		const int	s = i8_part_sum(rows, queries, kp, picked[slot], q, item - slot * parts);
 
 		if ((threadIdx.x & 63) < 32)
-			cand[slot * 32 + (threadIdx.x & 31)] = v;
+			atomicAdd(&sum[slot * 32 + (threadIdx.x & 31)], s);
 	}
 	__syncthreads();
+	for (uint32_t i = threadIdx.x; i < kk * 32; i += NT)
+		sum[i] = __float_as_int(i8_row_score(o, i == threadIdx.x ? first : i8_row(o, picked[i / 32], i % 32, q), sum[i], qs));
+	__syncthreads();
 	const uint32_t m = i8_select(S, [&](uint32_t i, float &v, uint32_t &id) -> bool {
-		v = cand[i];
+		v = __int_as_float(sum[i]);
 		id = picked[i / 32] * 32 + i % 32;
 		return v > I8_NINF;
 	}, kk * 32, k, floor);
@@ -1139,7 +1175,7 @@ k_i8_finish(const unsigned char *__restrict__ rows, const unsigned char *__restr
 	i8_results<NT>(S.list, m, k, ids + (size_t) q * k, scores + (size_t) q * k);
 }
 
-/* larger k: the rows of a query's blocks are scored by as many waves as there are blocks */
+/* otherwise every picked block of rows has a block of threads of its own */
 #define I8_NT 1024
 
 __global__ __launch_bounds__(I8_NT) void
@@ -1163,15 +1199,30 @@ __global__ __launch_bounds__(256) void
 k_i8_rescore(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, I8Out o, uint32_t k,
 			 const uint32_t *__restrict__ picked, const uint32_t *__restrict__ npicked, float *__restrict__ cand)
 {
-	const uint32_t slot = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const uint32_t q = blockIdx.y;
+	__shared__ int sum[32];
+	const uint32_t slot = blockIdx.x, q = blockIdx.y, i = threadIdx.x & 63;
 
 	if (slot >= npicked[q])
 		return;
-	const float v = i8_rescore(rows, queries, kp, o, picked[(size_t) q * k + slot], q);
+	const uint32_t rb = picked[(size_t) q * k + slot];
+	const uint32_t parts = (kp + 32 * I8_PART - 1) / (32 * I8_PART);
+	I8Row		w = {};
 
-	if ((threadIdx.x & 63) < 32)
-		cand[((size_t) q * k + slot) * 32 + (threadIdx.x & 31)] = v;
+	if (threadIdx.x < 32)
+	{
+		sum[i] = 0;
+		w = i8_row(o, rb, i, q);
+	}
+	__syncthreads();
+	int			s = 0;
+
+	for (uint32_t part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); part < parts; part += 4)
+		s += i8_part_sum(rows, queries, kp, rb, q, part);
+	if (i < 32)
+		atomicAdd(&sum[i], s);
+	__syncthreads();
+	if (threadIdx.x < 32)
+		cand[((size_t) q * k + slot) * 32 + i] = i8_row_score(o, w, sum[i], o.qscale[q]);
 }
 
 __global__ __launch_bounds__(I8_NT) void
@@ -1931,7 +1982,7 @@ ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const f
 		if (!i8_fused(t, m, k))
 		{
 			hipLaunchKernelGGL(k_i8_pick, dim3(m), dim3(I8_NT), 0, g.stream, o, (uint32_t) k, picked, npicked, floors);
-			hipLaunchKernelGGL(k_i8_rescore, dim3((k + 3) / 4, m), dim3(256), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, picked,
+			hipLaunchKernelGGL(k_i8_rescore, dim3(k, m), dim3(256), 0, g.stream, t->d_codes, qc, t->kp, o, (uint32_t) k, picked,
 							   npicked, cand);
 			hipLaunchKernelGGL(k_i8_best, dim3(m), dim3(I8_NT), 0, g.stream, cand, picked, npicked, floors, (uint32_t) k, d_ids + q0 * k,
 							   d_scores + q0 * k);
