@@ -575,6 +575,13 @@ i8_dma4(const void *base, uint32_t voff, uint32_t la)
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" :: "s"(la), "v"(voff), "s"(base));
 }
 
+/* the same from 64 unrelated addresses */
+__device__ __forceinline__ void
+i8_dma4_at(const void *p, uint32_t la)
+{
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off" :: "s"(la), "v"(p));
+}
+
 template <class T>
 __device__ __forceinline__ T *
 i8_uniform(T *p)
@@ -602,7 +609,7 @@ i8_lds(const void *p)
  * barrier that opens the next stage.  Tiles follow each other without a gap: the ring runs into the next tile of the
  * block, whose first operands are in registers when the sums of this one are written out.
  *
- * Row scales, query scales and biases of a tile come through LDS the same way, with the copies of its first stage: a load
+ * Row scales, query scales, biases and mask words of a tile come through LDS the same way, with the copies of its first stage: a load
  * of the wave's own would have to wait for every copy requested before it (requests retire in order).
  */
 #define I8_TR 8					/* blocks of rows in a tile */
@@ -620,15 +627,17 @@ template <int NWQ> struct I8Tile
 };
 
 template <int NWQ, class KIND>
-__global__ __launch_bounds__(128 * NWQ, 2) void
+__global__ __launch_bounds__(128 * NWQ, NWQ / 2) void
 k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrt, uint32_t nqt, I8Out o)
 {
 	typedef I8Tile<NWQ> TILE;
 	constexpr int QB = TILE::QB, PER = TILE::PER, WQ = I8_WQ;
+	static_assert(WQ == 2, "a wave's queries are its lanes in the copies of mask words");
 	__shared__ __attribute__((aligned(1024))) unsigned char ring[I8_NBUF * TILE::STAGE];
 	__shared__ __attribute__((aligned(1024))) float s_rs[I8_SLOTS][256];
 	__shared__ __attribute__((aligned(1024))) float s_qs[I8_SLOTS][256];
 	__shared__ __attribute__((aligned(1024))) float s_bias[KIND::BIAS ? I8_SLOTS : 1][256];
+	__shared__ __attribute__((aligned(1024))) uint32_t s_mask[KIND::MASK ? I8_SLOTS : 1][KIND::MASK ? TILE::NW : 1][4][64];
 	const int	lane = threadIdx.x & 63;
 	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int	wq = wave % NWQ, wr = wave / NWQ;
@@ -669,6 +678,17 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 		if (KIND::BIAS && wave < 4)
 			i8_dma4(i8_uniform(o.bias + (size_t) c_rt * 256), min(wave * 64u + lane, o.n - 1 - c_rt * 256) * 4,
 					i8_lds(s_bias) + c_slot * 1024 + wave * 256);
+		if (KIND::MASK)
+		{
+			/* the words of this wave's 64 queries, a lane each, for its four blocks of rows (the last query's and the last
+			 * block's again behind them: padding rows never take part, and nobody asks for padding queries) */
+			const uint32_t q = min((c_qt * QB + wq * WQ) * 32 + lane, o.nq - 1), nw = (o.n + 31) / 32;
+			const uint32_t *m = o.mask + (int64_t) q * o.mask_stride;
+
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				i8_dma4_at(m + min(c_rt * I8_TR + wr * 4 + i, nw - 1), i8_lds(s_mask) + ((c_slot * TILE::NW + wave) * 4 + i) * 256);
+		}
 	};
 	auto		c_copy = [&](int i) {
 		const int	c = wave * PER + i;			/* KiB c of the stage: block c / 2, half c % 2 */
@@ -794,7 +814,7 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 				for (int i = 0; i < 4; i++)
 					m[i] = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs[slot] + (wr * 4 + i) * 32,
 																s_bias[KIND::BIAS ? slot : 0] + (wr * 4 + i) * 32,
-																KIND::MASK ? i8_mask_word(o, rb0 + i, q) : 0u,
+																KIND::MASK ? s_mask[KIND::MASK ? slot : 0][KIND::MASK ? wave : 0][i][t * 32 + (lane & 31)] : 0u,
 																q < o.nq ? qs : 1.0f, acc[i][t]);
 				if (q < o.nq && lane < 32)
 				{
@@ -1830,8 +1850,10 @@ i8_tile_launch(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
 {
 	typedef I8Tile<NWQ> TILE;
 	const uint32_t nrt = (o.n + 255) / 256, nqt = (o.nq + 32 * TILE::QB - 1) / (32 * TILE::QB);
-	/* eight waves a compute unit, its blocks in whole rounds of the XCDs, and no more blocks than have a tile */
-	const uint32_t blocks = std::min(((uint32_t) g.num_cus & ~7u) * (8 / TILE::NW), (nrt + 7) / 8 * 8 * nqt);
+	/* as many blocks as the compute units hold (the narrow tile's LDS fits twice without biases and masks), in whole rounds of
+	 * the XCDs, and no more than have a tile */
+	const uint32_t per_cu = NWQ == 2 && !KIND::BIAS && !KIND::MASK ? 2 : 1;
+	const uint32_t blocks = std::min(((uint32_t) g.num_cus & ~7u) * per_cu, (nrt + 7) / 8 * 8 * nqt);
 
 	hipLaunchKernelGGL((k_i8_tile<NWQ, KIND>), dim3(blocks), dim3(64 * TILE::NW), 0, g.stream, t->d_codes, queries, t->kp, nrt, nqt, o);
 }
@@ -1841,12 +1863,16 @@ static int
 i8_multiply_kind(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
 {
 	const uint32_t nrb = (o.n + 31) / 32, nqb = (o.nq + 31) / 32;
+	const uint64_t nrt = (o.n + 255) / 256, w128 = (o.nq + 127) / 128, w256 = (o.nq + 255) / 256;
 
-	if (o.nq > 128)
-		i8_tile_launch<4, KIND>(t, queries, o);
-	else if (o.nq > 64)
-		i8_tile_launch<2, KIND>(t, queries, o);
-	else
+	/*
+	 * Up to 64 queries the table's bytes are what counts, and the stream reads them as fast as memory gives them.  Above, a
+	 * tile pays where there are enough of them to cover its start (scores of fp16; stream / 128-query tile / 256-query tile in
+	 * us): 96 x 16000 x 768 10.6 / 11.0 / 14.2, 256 x 16000 x 768 14.9 / 12.4 / 15.0, 96 x 64000 x 64 7.5 / 8.6 / 9.7, 256 x 64000
+	 * x 64 11.9 / 11.3 / 11.2.  The wide tile does a fifth more per query of its width (512 x 256000 x 768: 257 / 163 / 133) but
+	 * wants a tile for every compute unit (512 x 16000 x 768: 20.2 / 14.5 / 17.1).
+	 */
+	if (o.nq <= 64 || nrt * w128 * (t->kp + 128) <= 80000)
 	{
 		if (nqb == 1)
 			hipLaunchKernelGGL((k_i8_stream<1, KIND>), dim3((nrb + 3) / 4), dim3(256), 0, g.stream, t->d_codes, queries, t->kp, nrb, o);
@@ -1854,6 +1880,10 @@ i8_multiply_kind(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &
 			hipLaunchKernelGGL((k_i8_stream<2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
 							   nrb, o);
 	}
+	else if (nrt * w256 >= (uint32_t) g.num_cus && 10 * w256 * 2 <= 12 * w128)
+		i8_tile_launch<4, KIND>(t, queries, o);
+	else
+		i8_tile_launch<2, KIND>(t, queries, o);
 	HIP_TRY(hipGetLastError());
 	return NDBHIP_OK;
 }

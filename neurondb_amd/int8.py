@@ -36,6 +36,10 @@ class _Torch:
         self.words = (torch.int32, torch.uint32) if hasattr(torch, "uint32") else (torch.int32,)
         self.device = torch.device("cuda", _lib._device)
         self.lib = lib()
+        # torch's own short cut to the current stream's handle (0.1 us, against 1.7 us through a Stream object)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        index = _lib._device
+        self.stream = (lambda: raw(index)) if raw else (lambda: torch.cuda.current_stream(index).cuda_stream)
 
 
 _state = None
@@ -62,7 +66,7 @@ def _call(fn, *args):
     T = _state
     swap = T.lib.ndbhip_swap_thread_stream
     ref = _previous.ref
-    check(swap(T.torch.cuda.current_stream(T.device).cuda_stream or STREAM_LEGACY, ref))
+    check(swap(T.stream() or STREAM_LEGACY, ref))
     prev = _previous.p.value
     try:
         rc = fn(*args)
