@@ -57,10 +57,27 @@ template <> struct I8Elem<__hip_bfloat16>
 	static __device__ __forceinline__ __hip_bfloat16 store(float v) { return __float2bfloat16(v); }
 };
 
+/* N neighbouring elements in one access.  Global memory takes any alignment (an odd number of halves a row costs nothing
+ * but the lines that straddle), so there is one path for all strides. */
 template <class T, int N> struct alignas(sizeof(T) * N) I8Vec
 {
 	T			v[N];
 };
+template <class T, int N>
+__device__ __forceinline__ I8Vec<T, N>
+i8_get(const void *p)
+{
+	I8Vec<T, N> v;
+
+	__builtin_memcpy(&v, p, sizeof(v));
+	return v;
+}
+template <class T, int N>
+__device__ __forceinline__ void
+i8_put(void *p, const I8Vec<T, N> &v)
+{
+	__builtin_memcpy(p, &v, sizeof(v));
+}
 
 /* ================================================================== */
 /* quantise / dequantise                                               */
@@ -86,8 +103,8 @@ i8_byte(float x, float inv)
  */
 template <class T, bool BLOCKED, int CH>
 __global__ __launch_bounds__(256) void
-k_i8_quantize(const T *__restrict__ x, int64_t nrows, int64_t nrows_out, int dim, int64_t xstride, int lanes_log2, int xvec,
-			  unsigned char *__restrict__ codes, int64_t cstride, int cvec, uint32_t kp, float *__restrict__ scales)
+k_i8_quantize(const T *__restrict__ x, int64_t nrows, int64_t nrows_out, int dim, int64_t xstride, int lanes_log2,
+			  unsigned char *__restrict__ codes, int64_t cstride, uint32_t kp, float *__restrict__ scales)
 {
 	constexpr int VEC = 16 / sizeof(T);
 	const int	L = 1 << lanes_log2;
@@ -98,9 +115,9 @@ k_i8_quantize(const T *__restrict__ x, int64_t nrows, int64_t nrows_out, int dim
 	const int	step = L * VEC;
 
 	auto		load = [&](int e, float (&f)[VEC]) {
-		if (real && xvec && e + VEC <= dim)
+		if (real && e + VEC <= dim)
 		{
-			const I8Vec<T, VEC> v = *(const I8Vec<T, VEC> *) (p + e);
+			const I8Vec<T, VEC> v = i8_get<T, VEC>(p + e);
 
 #pragma unroll
 			for (int i = 0; i < VEC; i++)
@@ -148,33 +165,21 @@ k_i8_quantize(const T *__restrict__ x, int64_t nrows, int64_t nrows_out, int dim
 
 	unsigned char *out = BLOCKED ? codes + (size_t) (row >> 5) * 32u * kp + (row & 31) * 16u : codes + row * cstride;
 	auto		put = [&](int e, const float (&f)[VEC]) {
-		uint32_t	w[VEC / 4];
+		I8Vec<uint32_t, VEC / 4> w;
 
 #pragma unroll
 		for (int i = 0; i < VEC / 4; i++)
-			w[i] = live ? i8_byte(f[4 * i], inv) | i8_byte(f[4 * i + 1], inv) << 8 | i8_byte(f[4 * i + 2], inv) << 16 |
+			w.v[i] = live ? i8_byte(f[4 * i], inv) | i8_byte(f[4 * i + 1], inv) << 8 | i8_byte(f[4 * i + 2], inv) << 16 |
 				i8_byte(f[4 * i + 3], inv) << 24 : 0u;
 		if (BLOCKED)
-		{
-			unsigned char *o = out + (size_t) (e >> 4) * 512u + (e & 15);
-
-			if (VEC == 4)
-				*(uint32_t *) o = w[0];
-			else
-				*(uint2 *) o = make_uint2(w[0], w[VEC / 4 - 1]);
-		}
-		else if (cvec && e + VEC <= dim)
-		{
-			if (VEC == 4)
-				*(uint32_t *) (out + e) = w[0];
-			else
-				*(uint2 *) (out + e) = make_uint2(w[0], w[VEC / 4 - 1]);
-		}
+			*(I8Vec<uint32_t, VEC / 4> *) (out + (size_t) (e >> 4) * 512u + (e & 15)) = w;
+		else if (e + VEC <= dim)
+			i8_put(out + e, w);
 		else
 #pragma unroll
 			for (int i = 0; i < VEC; i++)
 				if (e + i < dim)
-					out[e + i] = (unsigned char) (w[i / 4] >> (8 * (i % 4)));
+					out[e + i] = (unsigned char) (w.v[i / 4] >> (8 * (i % 4)));
 	};
 	const int	end = BLOCKED ? (int) kp : dim;
 
@@ -202,8 +207,8 @@ k_i8_quantize(const T *__restrict__ x, int64_t nrows, int64_t nrows_out, int dim
 /* byte * scale in fp32, rounded once more where the output has 16 bits; a lane takes four elements at a time, CH loads ahead */
 template <class T>
 __global__ __launch_bounds__(256) void
-k_i8_dequantize(const int8_t *__restrict__ codes, int64_t cstride, int cvec, const float *__restrict__ scales, int64_t nrows, int dim,
-				int lanes_log2, T *__restrict__ out, int64_t ostride, int ovec)
+k_i8_dequantize(const int8_t *__restrict__ codes, int64_t cstride, const float *__restrict__ scales, int64_t nrows, int dim,
+				int lanes_log2, T *__restrict__ out, int64_t ostride)
 {
 	constexpr int CH = 4;
 	const int	L = 1 << lanes_log2;
@@ -226,8 +231,8 @@ k_i8_dequantize(const int8_t *__restrict__ codes, int64_t cstride, int cvec, con
 			const int	e = e0 + u * 4 * L;
 
 			w[u] = 0;
-			if (cvec && e + 4 <= dim)
-				w[u] = *(const uint32_t *) (c + e);
+			if (e + 4 <= dim)
+				w[u] = i8_get<uint32_t, 1>(c + e).v[0];
 			else
 #pragma unroll
 				for (int i = 0; i < 4; i++)
@@ -242,8 +247,8 @@ k_i8_dequantize(const int8_t *__restrict__ codes, int64_t cstride, int cvec, con
 #pragma unroll
 			for (int i = 0; i < 4; i++)
 				v.v[i] = I8Elem<T>::store((float) (int8_t) (w[u] >> (8 * i)) * s);
-			if (ovec && e + 4 <= dim)
-				*(I8Vec<T, 4> *) (o + e) = v;
+			if (e + 4 <= dim)
+				i8_put(o + e, v);
 			else
 #pragma unroll
 				for (int i = 0; i < 4; i++)
@@ -256,7 +261,7 @@ k_i8_dequantize(const int8_t *__restrict__ codes, int64_t cstride, int cvec, con
 /* rows of bytes <-> the block layout, 16 bytes a thread (neighbouring threads: neighbouring slices of a row) */
 template <bool PACK>
 __global__ __launch_bounds__(256) void
-k_i8_blocks(const unsigned char *__restrict__ src, unsigned char *__restrict__ dst, int64_t stride, int vec, int64_t nrows, int64_t nrows_out,
+k_i8_blocks(const unsigned char *__restrict__ src, unsigned char *__restrict__ dst, int64_t stride, int64_t nrows, int64_t nrows_out,
 			int dim, uint32_t kp, const float *__restrict__ sin, float *__restrict__ sout)
 {
 	const uint32_t slices = kp / 16;
@@ -267,32 +272,32 @@ k_i8_blocks(const unsigned char *__restrict__ src, unsigned char *__restrict__ d
 	if (row >= nrows_out)
 		return;
 	const size_t blk = (size_t) (row >> 5) * 32u * kp + (row & 31) * 16u + (size_t) (e >> 4) * 512u;
-	union { uint4 q; unsigned char b[16]; } u;
+	I8Vec<unsigned char, 16> u;
 
 	if (PACK)
 	{
 		const unsigned char *s = src + row * stride + e;
 
-		u.q = make_uint4(0, 0, 0, 0);
-		if (row < nrows && vec && e + 16 <= dim)
-			u.q = *(const uint4 *) s;
-		else if (row < nrows)
+		if (row < nrows && e + 16 <= dim)
+			u = i8_get<unsigned char, 16>(s);
+		else
+#pragma unroll
 			for (int i = 0; i < 16; i++)
-				if (e + i < dim)
-					u.b[i] = s[i];
-		*(uint4 *) (dst + blk) = u.q;
+				u.v[i] = row < nrows && e + i < dim ? s[i] : 0;
+		*(I8Vec<unsigned char, 16> *) (dst + blk) = u;
 	}
 	else
 	{
 		unsigned char *d = dst + row * stride + e;
 
-		u.q = *(const uint4 *) (src + blk);
-		if (vec && e + 16 <= dim)
-			*(uint4 *) d = u.q;
+		u = *(const I8Vec<unsigned char, 16> *) (src + blk);
+		if (e + 16 <= dim)
+			i8_put(d, u);
 		else
+#pragma unroll
 			for (int i = 0; i < 16; i++)
 				if (e + i < dim)
-					d[i] = u.b[i];
+					d[i] = u.v[i];
 	}
 	if (e == 0)
 		sout[row] = row < nrows ? sin[row] : __builtin_nanf("");
@@ -1286,9 +1291,9 @@ k_i8_none(int64_t *__restrict__ ids, float *__restrict__ scores, uint64_t n)
  */
 template <class T, int U>
 __global__ __launch_bounds__(256) void
-k_scores_adjust(const T *scores, int64_t stride, int64_t n, int svec, const int64_t *__restrict__ seen_off,
+k_scores_adjust(const T *scores, int64_t stride, int64_t n, const int64_t *__restrict__ seen_off,
 				const int32_t *__restrict__ seen_ids, const float *__restrict__ penalties, const float *__restrict__ bias, int64_t bias_stride,
-				int bvec, const uint32_t *__restrict__ mask, int64_t mask_stride, T *out, int64_t ostride, int q0)
+				const uint32_t *__restrict__ mask, int64_t mask_stride, T *out, int64_t ostride, int q0)
 {
 	constexpr int VEC = 16 / sizeof(T), COLS = 256 * VEC * U;
 	__shared__ __attribute__((aligned(16))) uint32_t cnt[COLS];
@@ -1311,8 +1316,8 @@ k_scores_adjust(const T *scores, int64_t stride, int64_t n, int svec, const int6
 		word[u] = 0xFFFFFFFFu;
 		if (e < m)
 		{
-			if (svec && e + VEC <= m)
-				v[u] = *(const I8Vec<T, VEC> *) (src + e);
+			if (e + VEC <= m)
+				v[u] = i8_get<T, VEC>(src + e);
 			else
 #pragma unroll
 				for (int i = 0; i < VEC; i++)
@@ -1320,10 +1325,16 @@ k_scores_adjust(const T *scores, int64_t stride, int64_t n, int svec, const int6
 						v[u].v[i] = src[e + i];
 			if (mv)
 				word[u] = mv[e / 32] >> (e % 32);
-			if (bv && bvec && e + VEC <= m)
+			if (bv && e + VEC <= m)
 #pragma unroll
 				for (int i = 0; i < VEC; i += 4)
-					*(float4 *) &add[u][i] = *(const float4 *) (bv + e + i);
+				{
+					const I8Vec<float, 4> b = i8_get<float, 4>(bv + e + i);
+
+#pragma unroll
+					for (int j = 0; j < 4; j++)
+						add[u][i + j] = b.v[j];
+				}
 			else if (bv)
 #pragma unroll
 				for (int i = 0; i < VEC; i++)
@@ -1392,8 +1403,8 @@ k_scores_adjust(const T *scores, int64_t stride, int64_t n, int svec, const int6
 				s[i] = I8_NINF;
 			v[u].v[i] = I8Elem<T>::store(s[i]);
 		}
-		if (svec && e + VEC <= m)
-			*(I8Vec<T, VEC> *) (dst + e) = v[u];
+		if (e + VEC <= m)
+			i8_put(dst + e, v[u]);
 		else
 #pragma unroll
 			for (int i = 0; i < VEC; i++)
@@ -1425,12 +1436,6 @@ i8_type_size(int dtype)
 	return dtype == NDBHIP_F32 ? 4 : dtype == NDBHIP_F16 || dtype == NDBHIP_BF16 ? 2 : dtype == NDBHIP_I8 ? 1 : 0;
 }
 
-static bool
-i8_aligned(const void *p, int64_t stride_bytes, unsigned to)
-{
-	return ((uintptr_t) p % to) == 0 && (stride_bytes % to) == 0;
-}
-
 /* lanes for a row of `units` lane-loads, as a power of two's exponent: the smallest that covers it, at most a wave */
 static int
 i8_lanes_log2(int64_t units)
@@ -1456,8 +1461,6 @@ i8_quantize_launch(const void *d_x, int64_t nrows, int64_t nrows_out, int dim, i
 {
 	constexpr int VEC = 16 / sizeof(T);
 	const int	ll = i8_lanes_log2((dim + VEC - 1) / VEC);
-	const int	xvec = i8_aligned(d_x, xstride * (int64_t) sizeof(T), 16);
-	const int	cvec = i8_aligned(codes, cstride, VEC);
 	const int64_t slab = i8_slab_rows(dim);
 
 	for (int64_t r0 = 0; r0 < nrows_out; r0 += slab)
@@ -1466,8 +1469,8 @@ i8_quantize_launch(const void *d_x, int64_t nrows, int64_t nrows_out, int dim, i
 
 		/* (a launch of padding rows alone reads nothing; its pointer stays at the first row) */
 		hipLaunchKernelGGL((k_i8_quantize<T, BLOCKED, 4>), dim3((unsigned) ((m + (256 >> ll) - 1) / (256 >> ll))), dim3(256), 0, g.stream,
-						   (const T *) d_x + (real ? r0 * xstride : 0), real, m, dim, xstride, ll, xvec,
-						   codes + r0 * (BLOCKED ? (int64_t) kp : cstride), cstride, cvec, kp, scales + r0);
+						   (const T *) d_x + (real ? r0 * xstride : 0), real, m, dim, xstride, ll,
+						   codes + r0 * (BLOCKED ? (int64_t) kp : cstride), cstride, kp, scales + r0);
 	}
 	HIP_TRY(hipGetLastError());
 	return NDBHIP_OK;
@@ -1498,8 +1501,7 @@ i8_pack(const void *codes, int64_t stride, const float *scales, int64_t nrows, i
 		const uint64_t units = (uint64_t) m * (kp / 16);
 
 		hipLaunchKernelGGL(k_i8_blocks<true>, dim3((unsigned) ((units + 255) / 256)), dim3(256), 0, g.stream,
-						   (const unsigned char *) codes + (real ? r0 * stride : 0), dst + r0 * kp, stride, (int) i8_aligned(codes, stride, 16),
-						   real, m, dim, kp, scales + (real ? r0 : 0), sout + r0);
+						   (const unsigned char *) codes + (real ? r0 * stride : 0), dst + r0 * kp, stride, real, m, dim, kp, scales + (real ? r0 : 0), sout + r0);
 	}
 	HIP_TRY(hipGetLastError());
 	return NDBHIP_OK;
@@ -1533,8 +1535,7 @@ i8_dequantize_launch(const int8_t *codes, int64_t cstride, const float *scales, 
 		const int64_t m = std::min(slab, nrows - r0);
 
 		hipLaunchKernelGGL(k_i8_dequantize<T>, dim3((unsigned) ((m + per - 1) / per)), dim3(256), 0, g.stream, codes + r0 * cstride, cstride,
-						   (int) i8_aligned(codes, cstride, 4), scales + r0, m, dim, ll, (T *) out + r0 * ostride, ostride,
-						   (int) i8_aligned(out, ostride * (int64_t) sizeof(T), 4 * sizeof(T)));
+						   scales + r0, m, dim, ll, (T *) out + r0 * ostride, ostride);
 	}
 }
 
@@ -1720,8 +1721,7 @@ ndbhip_i8_export_device(const ndbhip_i8 *t, int8_t *d_codes, int64_t codes_strid
 		const uint64_t units = (uint64_t) m * (t->kp / 16);
 
 		hipLaunchKernelGGL(k_i8_blocks<false>, dim3((unsigned) ((units + 255) / 256)), dim3(256), 0, g.stream,
-						   (const unsigned char *) t->d_codes + r0 * t->kp, (unsigned char *) d_codes + r0 * codes_stride, codes_stride,
-						   (int) i8_aligned(d_codes, codes_stride, 16), m, m, t->dim, t->kp, t->d_scales + r0, d_scales + r0);
+						   (const unsigned char *) t->d_codes + r0 * t->kp, (unsigned char *) d_codes + r0 * codes_stride, codes_stride, m, m, t->dim, t->kp, t->d_scales + r0, d_scales + r0);
 	}
 	HIP_TRY(hipGetLastError());
 	return NDBHIP_OK;
@@ -2095,19 +2095,17 @@ scores_adjust_launch(const void *s, int64_t stride, int nq, int64_t n, const int
 	/* columns a block takes: many scores 4096 (fp32) or 8192 (16 bits), which halves the list's reads; else half of that */
 	constexpr int VEC = 16 / sizeof(T);
 	const int	u = (int64_t) nq * n >= ((int64_t) 4 << 20) ? 4 : 2, cols = 256 * VEC * u;
-	const int	vec = i8_aligned(s, stride * (int64_t) sizeof(T), 16) && i8_aligned(out, ostride * (int64_t) sizeof(T), 16);
-	const int	bvec = i8_aligned(bias, bias_stride * 4, 16);
 
 	for (int q0 = 0; q0 < nq; q0 += 65535)
 	{
 		const dim3	grid((unsigned) ((n + cols - 1) / cols), std::min(65535, nq - q0));
 
 		if (u == 4)
-			hipLaunchKernelGGL((k_scores_adjust<T, 4>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, vec, off, ids, pen, bias,
-							   bias_stride, bvec, mask, mask_stride, (T *) out, ostride, q0);
+			hipLaunchKernelGGL((k_scores_adjust<T, 4>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, off, ids, pen, bias,
+							   bias_stride, mask, mask_stride, (T *) out, ostride, q0);
 		else
-			hipLaunchKernelGGL((k_scores_adjust<T, 2>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, vec, off, ids, pen, bias,
-							   bias_stride, bvec, mask, mask_stride, (T *) out, ostride, q0);
+			hipLaunchKernelGGL((k_scores_adjust<T, 2>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, off, ids, pen, bias,
+							   bias_stride, mask, mask_stride, (T *) out, ostride, q0);
 	}
 }
 

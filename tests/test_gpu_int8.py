@@ -289,6 +289,38 @@ def test_search(nq, n, dim, k, what):
     same(sc, ref[1])
 
 
+@pytest.mark.parametrize("nq,n,dim,k", [(130, 60_001, 33, 10), (65, 100_003, 64, 3), (200, 70_001, 40, 129), (384, 40_007, 130, 20), (700, 33_000, 8, 5),
+                                        (257, 9000, 2049, 12)])
+@pytest.mark.parametrize("what", ["plain", "bias", "mask1", "mask", "all"])
+def test_search_and_product_in_many_tiles(nq, n, dim, k, what):
+    """batches whose product takes LDS tiles, narrow and wide ones, with rows, queries and dimensions that fill none"""
+    rows, q = rand(n + k, n, dim), rand(nq, nq, dim)
+    rows[:: n // 9] = rows[n // 2].clone()
+    t = nd.Int8Table(dim)
+    t.load(rows.cuda())
+    bias = rand(9, n) if what in ("bias", "all") else None
+    mask = None
+    if what in ("mask", "mask1", "all"):
+        bits = np.random.default_rng(n).random((1 if what == "mask1" else nq, n)) < 0.05
+        bits[-1, : n // 2] = False
+        if what != "mask1":
+            bits[nq // 2] = False
+        mask = pack(bits)
+    s = scores_of(*quantise(q), *quantise(rows), bias=bias)
+    if mask is None:
+        for out_t in (F32, F16):
+            same(t.scores(q.cuda(), bias=None if bias is None else bias.cuda(), dtype=out_t), s.to(out_t))
+    at = [0, 1, nq // 2, nq - 2, nq - 1]
+    ref = best(s[at], k, mask if what in ("plain", "bias", "mask1") else mask[at])
+    ids, sc = t.search(q.cuda(), k, bias=None if bias is None else bias.cuda(), mask=None if mask is None else mask.cuda())
+    same(ids[at], ref[0])
+    same(sc[at], ref[1])
+    # every query: the k best, recomputed from the scores on the device
+    if mask is not None:
+        s = s.masked_fill(~unpack(mask, n), -math.inf)
+    same(sc, s.cuda().topk(k, 1).values)
+
+
 @pytest.mark.parametrize("nq,n,k", [(1, 70_000, 10), (4, 3000, 1024), (70, 9000, 50), (300, 3000, 200)])
 def test_search_where_every_score_is_equal(nq, n, k):
     for rows in (torch.ones(n, 32), torch.zeros(n, 32), torch.ones(n, 32) * (torch.arange(n) % 2 * 2 - 1)[:, None]):
