@@ -920,13 +920,13 @@ i8_sort(I8Select<NT, CAP> &S, uint32_t m)
 }
 
 /*
- * The min(k, valid) best of the elements f(i, score, id) -> takes part, i = 0 .. n - 1, in order in S.list; returns how
- * many.  At least min(k, valid) elements have to reach `floor`.  Where more do than the list holds (many equal scores), the
+ * The elements f(i, score, id) -> takes part, i = 0 .. n - 1, that reach `floor`, as words in S.list in no order; returns how
+ * many.  At least min(k, valid) have to reach it.  Where more do than the list holds (many equal scores), the k best: the
  * k-th score is found by radix selection, and the k-th id among its equals.  Ends with a barrier.
  */
 template <int NT, int CAP, class F>
 __device__ uint32_t
-i8_select(I8Select<NT, CAP> &S, F f, uint32_t n, uint32_t k, float floor)
+i8_gather(I8Select<NT, CAP> &S, F f, uint32_t n, uint32_t k, float floor)
 {
 	if (threadIdx.x == 0)
 		S.cnt = 0;
@@ -945,68 +945,116 @@ i8_select(I8Select<NT, CAP> &S, F f, uint32_t n, uint32_t k, float floor)
 		}
 	}
 	__syncthreads();
-	uint32_t	m = S.cnt;
+	const uint32_t m = S.cnt;
 
-	if (m > CAP)
+	if (m <= CAP)
+		return m;
+
+	uint32_t	T, less, kk, eq, T2 = ~0u;
+
+	block_radix_select([&](uint32_t i, uint32_t &bits) -> bool {
+		float		v;
+		uint32_t	id;
+		const bool	ok = f(i, v, id);
+
+		bits = __float_as_uint(-v);
+		return ok;
+	}, n, k, S.hist, S.sh, T, less, kk, eq);
+	if (eq > kk - less)
 	{
-		uint32_t	T, less, kk, eq, T2 = ~0u;
+		uint32_t	l2, k2, e2;
 
 		block_radix_select([&](uint32_t i, uint32_t &bits) -> bool {
 			float		v;
-			uint32_t	id;
-			const bool	ok = f(i, v, id);
+			const bool	ok = f(i, v, bits);
 
-			bits = __float_as_uint(-v);
-			return ok;
-		}, n, k, S.hist, S.sh, T, less, kk, eq);
-		if (eq > kk - less)
-		{
-			uint32_t	l2, k2, e2;
-
-			block_radix_select([&](uint32_t i, uint32_t &bits) -> bool {
-				float		v;
-				const bool	ok = f(i, v, bits);
-
-				return ok && ndb_key_from_bits(__float_as_uint(-v)) == T;
-			}, n, kk - less, S.hist, S.sh, T2, l2, k2, e2);
-		}
-		if (threadIdx.x == 0)
-			S.cnt = 0;
-		__syncthreads();
-		for (uint32_t i = threadIdx.x; i < n; i += NT)
-		{
-			float		v;
-			uint32_t	id;
-
-			if (!f(i, v, id))
-				continue;
-			const uint32_t key = ndb_key_from_bits(__float_as_uint(-v));
-
-			/* (ids are below 2^31: as keys of floats they keep their order) */
-			if (key < T || (key == T && ndb_key_from_bits(id) <= T2))
-				S.list[atomicAdd(&S.cnt, 1u)] = i8_word(v, id);
-		}
-		__syncthreads();
-		m = kk;
+			return ok && ndb_key_from_bits(__float_as_uint(-v)) == T;
+		}, n, kk - less, S.hist, S.sh, T2, l2, k2, e2);
 	}
+	if (threadIdx.x == 0)
+		S.cnt = 0;
+	__syncthreads();
+	for (uint32_t i = threadIdx.x; i < n; i += NT)
+	{
+		float		v;
+		uint32_t	id;
+
+		if (!f(i, v, id))
+			continue;
+		const uint32_t key = ndb_key_from_bits(__float_as_uint(-v));
+
+		/* (ids are below 2^31: as keys of floats they keep their order) */
+		if (key < T || (key == T && ndb_key_from_bits(id) <= T2))
+			S.list[atomicAdd(&S.cnt, 1u)] = i8_word(v, id);
+	}
+	__syncthreads();
+	return kk;
+}
+
+/* the min(k, valid) best of them in order; returns how many */
+template <int NT, int CAP, class F>
+__device__ uint32_t
+i8_select(I8Select<NT, CAP> &S, F f, uint32_t n, uint32_t k, float floor)
+{
+	const uint32_t m = i8_gather(S, f, n, k, floor);
+
 	i8_sort(S, m);
 	return min(m, k);
 }
 
 /*
- * The k best blocks of 32 rows of a query, in S.list; returns how many there are.  The floor of the first step: the
- * k-th largest of the maxima of 2k .. 4k groups of threads' quads.
+ * A floor under the k-th largest of top[0 .. groups), k <= groups <= 64 N, by one wave: the leading 20 bits of the
+ * largest key that k of them reach (sign, exponent and 11 bits of the mantissa: within 2^-11 below the k-th itself).
+ */
+template <int N>
+__device__ __forceinline__ float
+i8_floor(const float *top, uint32_t groups, uint32_t k)
+{
+	const int	lane = threadIdx.x & 63;
+	uint32_t	key[N], T = 0;
+
+#pragma unroll
+	for (int e = 0; e < N; e++)
+	{
+		const uint32_t i = e * 64 + lane;
+
+		/* (larger scores: larger keys; nothing: 0, which no threshold but 0 admits) */
+		key[e] = i < groups && top[i] > I8_NINF ? ndb_key_from_bits(__float_as_uint(top[i])) : 0u;
+	}
+	for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1)
+	{
+		uint32_t	c = 0;
+
+#pragma unroll
+		for (int e = 0; e < N; e++)
+			c += __popcll(__ballot(key[e] >= (T | bit)));
+		if (c >= k)
+			T |= bit;
+	}
+	if (T == 0)
+		return I8_NINF;
+	const float f = __uint_as_float((T & 0x80000000u) ? T ^ 0x80000000u : ~T);
+
+	return f == f ? f : I8_NINF;	/* (between -infinity's key and the smallest number's lie those of NaN) */
+}
+
+/*
+ * The k best blocks of 32 rows of a query, in S.list; returns how many there are.  The floor of every step: k of about 2k .. 4k
+ * groups of threads have a quad that reaches it.
  */
 template <int NT, int CAP>
 __device__ uint32_t
-i8_pick(I8Select<NT, CAP> &S, uint32_t *quads, const float *gm, const float *qm, uint32_t ng, uint32_t k)
+i8_pick(I8Select<NT, CAP> &S, uint32_t (&quads)[CAP], const float *gm, const float *qm, uint32_t ng, uint32_t k)
 {
 	const uint32_t nquad = (ng + 3) / 4;
+	const uint32_t span = min(nquad, (uint32_t) NT);
 	float		t = I8_NINF;
-	uint32_t	groups = max(NT / 64, 16);
+	uint32_t	size = 64;			/* threads of a group, neighbours in a wave */
 
-	while (groups < 2 * k && groups < NT)
-		groups <<= 1;
+	while (size > 1 && span < 2 * k * size)
+		size >>= 1;
+	const uint32_t groups = (span + size - 1) / size;
+
 	for (uint32_t i = threadIdx.x; i < nquad; i += 8 * NT)
 	{
 		float		v[8];
@@ -1018,64 +1066,35 @@ i8_pick(I8Select<NT, CAP> &S, uint32_t *quads, const float *gm, const float *qm,
 		for (int e = 0; e < 8; e++)
 			t = fmaxf(t, v[e]);
 	}
-	for (uint32_t off = 1; off < NT / groups; off <<= 1)
+	for (uint32_t off = 1; off < size; off <<= 1)
 		t = fmaxf(t, __shfl_xor(t, off, 64));
-	if (threadIdx.x % (NT / groups) == 0)
-		S.top[threadIdx.x / (NT / groups)] = t;
-	if (threadIdx.x == 0)
-		S.floor = I8_NINF;
+	if (threadIdx.x % size == 0)
+		S.top[threadIdx.x / size] = t;
 	__syncthreads();
-	if (k <= groups && groups <= 256)
+	if (threadIdx.x < 64)
 	{
-		if (threadIdx.x < groups)
-		{
-			const float mine = S.top[threadIdx.x];
-			uint32_t	r = 0;
+		const float f = k > groups ? I8_NINF : groups <= 64 ? i8_floor<1>(S.top, groups, k) : groups <= 256 ?
+			i8_floor<4>(S.top, groups, k) : i8_floor<NT / 64>(S.top, groups, k);
 
-			for (uint32_t j = 0; j < groups; j += 16)	/* (groups: at least 16; sixteen reads in flight, no branches) */
-			{
-				float		o[16];
-
-#pragma unroll
-				for (uint32_t e = 0; e < 16; e++)
-					o[e] = S.top[j + e];
-#pragma unroll
-				for (uint32_t e = 0; e < 16; e++)
-					r += (uint32_t) (o[e] > mine) | ((uint32_t) (o[e] == mine) & (uint32_t) (j + e < threadIdx.x));
-			}
-			if (r == k - 1)
-				S.floor = mine;
-		}
-		__syncthreads();
+		if (threadIdx.x == 0)
+			S.floor = f;
 	}
-	else if (k <= groups)
-	{
-		uint32_t	T, less, kk, eq;
-
-		block_radix_select([&](uint32_t i, uint32_t &bits) -> bool {
-			bits = __float_as_uint(-S.top[i]);
-			return S.top[i] > I8_NINF;
-		}, groups, k, S.hist, S.sh, T, less, kk, eq);
-		if (threadIdx.x == 0 && kk == k)
-			S.floor = i8_word_score((uint64_t) T << 32);
-		__syncthreads();
-	}
+	__syncthreads();
 	const float floor = S.floor;
-	const uint32_t nq4 = i8_select(S, [&](uint32_t i, float &v, uint32_t &id) -> bool {
+	const uint32_t m = i8_gather(S, [&](uint32_t i, float &v, uint32_t &id) -> bool {
 		v = qm[i];
 		id = i;
 		return v > I8_NINF;
 	}, nquad, k, floor);
-	const float floor2 = nq4 == k ? i8_word_score(S.list[k - 1]) : I8_NINF;
 
-	for (uint32_t i = threadIdx.x; i < nq4; i += NT)
+	for (uint32_t i = threadIdx.x; i < m; i += NT)
 		quads[i] = (uint32_t) S.list[i];
 	__syncthreads();
 	return i8_select(S, [&](uint32_t i, float &v, uint32_t &id) -> bool {
 		id = quads[i / 4] * 4 + i % 4;
 		v = id < ng ? gm[id] : I8_NINF;
 		return v > I8_NINF;
-	}, nq4 * 4, k, floor2);
+	}, m * 4, k, floor);
 }
 
 /*
@@ -1162,7 +1181,7 @@ k_i8_finish(const unsigned char *__restrict__ rows, const unsigned char *__restr
 			int64_t *__restrict__ ids, float *__restrict__ scores)
 {
 	__shared__ I8Select<NT, 512> S;
-	__shared__ uint32_t picked[I8_FUSED_K];
+	__shared__ uint32_t picked[512];			/* (quads first) */
 	__shared__ int sum[I8_FUSED_K * 32];		/* (a score's bits take the place of its sum) */
 	const uint32_t q = blockIdx.x;
 	const float qs = o.qscale[q];
@@ -1207,7 +1226,7 @@ __global__ __launch_bounds__(I8_NT) void
 k_i8_pick(I8Out o, uint32_t k, uint32_t *__restrict__ picked, uint32_t *__restrict__ npicked, float *__restrict__ floors)
 {
 	__shared__ I8Select<I8_NT, 2048> S;
-	__shared__ uint32_t quads[NDBHIP_MAX_K];
+	__shared__ uint32_t quads[2048];
 	const uint32_t q = blockIdx.x;
 	const uint32_t kk = i8_pick(S, quads, o.gmax + (size_t) q * o.ngp, o.qmax + (size_t) q * (o.ngp / 4), (o.n + 31) / 32, k);
 
