@@ -802,12 +802,12 @@ int			ndbhip_i8_search(const ndbhip_i8 *t, const float *queries, int nq, const f
 /* Penalties, biases and masks over a matrix of scores [nq][n] (fp32, fp16 or bf16; arithmetic in fp32, rounded once), to
  * another matrix of the type or in place (d_out == d_scores with the same stride; no other overlap):
  *   seen       query q has been given ids d_seen_ids[d_seen_off[q] .. d_seen_off[q + 1]) before, in any order, an id once for
- *              every time; ids outside 0 .. n - 1 count for nothing.  d_penalties[q] = {repeat, presence, frequency}, repeat > 0.  For an id
+ *              every time; what lies outside the n_seen ids there are is not read, ids outside 0 .. n - 1 count for nothing.  d_penalties[q] = {repeat, presence, frequency}, repeat > 0.  For an id
  *              given c > 0 times: s = s > 0 ? s / repeat : s * repeat, then s = s - (presence + c * frequency).  d_seen_off NULL: none
  *   bias       s = s + bias; bias_stride from one query's to the next, 0 = one for all; NULL: none
  *   mask       bit 0: s = -infinity, whatever it was; as above; NULL: none */
 int			ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, int64_t stride, const int64_t *d_seen_off,
-										const int32_t *d_seen_ids, const float *d_penalties, const float *d_bias, int64_t bias_stride,
+										const int32_t *d_seen_ids, int64_t n_seen, const float *d_penalties, const float *d_bias, int64_t bias_stride,
 										const uint32_t *d_mask, int64_t mask_stride, void *d_out, int64_t out_stride);
 
 #ifdef __cplusplus

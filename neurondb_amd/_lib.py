@@ -169,7 +169,7 @@ def lib():
         "ndbhip_i8_product_device": (i, [vp, vp, i, vp, i, i64, vp, vp, i, i64, vp, C.c_size_t]),
         "ndbhip_i8_search_device": (i, [vp, vp, i, vp, i, i64, vp, vp, i64, i, vp, vp, vp, C.c_size_t]),
         "ndbhip_i8_search": (i, [vp, vp, i, vp, vp, i64, i, vp, vp]),
-        "ndbhip_scores_adjust_device": (i, [vp, i, i, i64, i64, vp, vp, vp, vp, i64, vp, i64, vp, i64]),
+        "ndbhip_scores_adjust_device": (i, [vp, i, i, i64, i64, vp, vp, i64, vp, vp, i64, vp, i64, vp, i64]),
         "ndbhip_mfma_probe": (i, [vp, vp, vp, vp, i, i]),
         "ndbhip_mfma_probe_f32": (i, [vp, vp, vp, vp, i]),
         "ndbhip_debug_phases": (i, [vp]),

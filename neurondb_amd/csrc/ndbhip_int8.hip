@@ -1311,7 +1311,7 @@ k_i8_none(int64_t *__restrict__ ids, float *__restrict__ scores, uint64_t n)
 template <class T, int U>
 __global__ __launch_bounds__(256) void
 k_scores_adjust(const T *scores, int64_t stride, int64_t n, const int64_t *__restrict__ seen_off,
-				const int32_t *__restrict__ seen_ids, const float *__restrict__ penalties, const float *__restrict__ bias, int64_t bias_stride,
+				const int32_t *__restrict__ seen_ids, int64_t nseen, const float *__restrict__ penalties, const float *__restrict__ bias, int64_t bias_stride,
 				const uint32_t *__restrict__ mask, int64_t mask_stride, T *out, int64_t ostride, int q0)
 {
 	constexpr int VEC = 16 / sizeof(T), COLS = 256 * VEC * U;
@@ -1360,7 +1360,7 @@ k_scores_adjust(const T *scores, int64_t stride, int64_t n, const int64_t *__res
 					add[u][i] = e + i < m ? bv[e + i] : 0.0f;
 		}
 	}
-	const int64_t lo = seen_off ? seen_off[q] : 0, hi = seen_off ? seen_off[q + 1] : 0;
+	const int64_t lo = seen_off ? max(seen_off[q], (int64_t) 0) : 0, hi = seen_off ? min(seen_off[q + 1], nseen) : 0;
 	const bool	seen = hi > lo;
 	float		repeat = 1.0f, presence = 0.0f, frequency = 0.0f;
 
@@ -2108,7 +2108,7 @@ ndbhip_i8_search(const ndbhip_i8 *t, const float *queries, int nq, const float *
 
 template <class T>
 static void
-scores_adjust_launch(const void *s, int64_t stride, int nq, int64_t n, const int64_t *off, const int32_t *ids, const float *pen, const float *bias,
+scores_adjust_launch(const void *s, int64_t stride, int nq, int64_t n, const int64_t *off, const int32_t *ids, int64_t nids, const float *pen, const float *bias,
 					 int64_t bias_stride, const uint32_t *mask, int64_t mask_stride, void *out, int64_t ostride)
 {
 	/* columns a block takes: many scores 4096 (fp32) or 8192 (16 bits), which halves the list's reads; else half of that */
@@ -2120,17 +2120,17 @@ scores_adjust_launch(const void *s, int64_t stride, int nq, int64_t n, const int
 		const dim3	grid((unsigned) ((n + cols - 1) / cols), std::min(65535, nq - q0));
 
 		if (u == 4)
-			hipLaunchKernelGGL((k_scores_adjust<T, 4>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, off, ids, pen, bias,
+			hipLaunchKernelGGL((k_scores_adjust<T, 4>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, off, ids, nids, pen, bias,
 							   bias_stride, mask, mask_stride, (T *) out, ostride, q0);
 		else
-			hipLaunchKernelGGL((k_scores_adjust<T, 2>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, off, ids, pen, bias,
+			hipLaunchKernelGGL((k_scores_adjust<T, 2>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, off, ids, nids, pen, bias,
 							   bias_stride, mask, mask_stride, (T *) out, ostride, q0);
 	}
 }
 
 extern "C" int
 ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, int64_t stride, const int64_t *d_seen_off,
-							const int32_t *d_seen_ids, const float *d_penalties, const float *d_bias, int64_t bias_stride,
+							const int32_t *d_seen_ids, int64_t n_seen, const float *d_penalties, const float *d_bias, int64_t bias_stride,
 							const uint32_t *d_mask, int64_t mask_stride, void *d_out, int64_t out_stride)
 {
 	if (dtype != NDBHIP_F32 && dtype != NDBHIP_F16 && dtype != NDBHIP_BF16)
@@ -2141,7 +2141,7 @@ ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, 
 		return fail(NDBHIP_ERR_INVALID, "bias_stride must be 0 (one bias) or at least n");
 	if (d_mask && mask_stride != 0 && mask_stride < (n + 31) / 32)
 		return fail(NDBHIP_ERR_INVALID, "mask_stride must be 0 (one mask) or at least a word for every 32 scores");
-	if (d_seen_off && (!d_seen_ids || !d_penalties))
+	if (d_seen_off && (n_seen < 0 || !d_seen_ids || !d_penalties))
 		return fail(NDBHIP_ERR_INVALID, "offsets without ids or penalties");
 	if (nq > 0 && n > 0 && (!d_scores || !d_out))
 		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
@@ -2151,13 +2151,13 @@ ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, 
 	if (nq == 0 || n == 0)
 		return NDBHIP_OK;
 	if (dtype == NDBHIP_F32)
-		scores_adjust_launch<float>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, d_penalties, d_bias, bias_stride, d_mask, mask_stride,
+		scores_adjust_launch<float>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, n_seen, d_penalties, d_bias, bias_stride, d_mask, mask_stride,
 									d_out, out_stride);
 	else if (dtype == NDBHIP_F16)
-		scores_adjust_launch<__half>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, d_penalties, d_bias, bias_stride, d_mask, mask_stride,
+		scores_adjust_launch<__half>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, n_seen, d_penalties, d_bias, bias_stride, d_mask, mask_stride,
 									 d_out, out_stride);
 	else
-		scores_adjust_launch<__hip_bfloat16>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, d_penalties, d_bias, bias_stride, d_mask,
+		scores_adjust_launch<__hip_bfloat16>(d_scores, stride, nq, n, d_seen_off, d_seen_ids, n_seen, d_penalties, d_bias, bias_stride, d_mask,
 											 mask_stride, d_out, out_stride);
 	HIP_TRY(hipGetLastError());
 	return NDBHIP_OK;

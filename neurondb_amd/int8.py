@@ -189,6 +189,7 @@ def adjust_scores(scores, seen=None, penalties=None, bias=None, mask=None, out=N
         out = T.torch.empty((nq, n), dtype=scores.dtype, device=T.device)
         ostride = n
     off = ids = None
+    nids = 0
     if (seen is None) != (penalties is None):
         raise _bad("seen and penalties go together")
     if seen is not None:
@@ -198,11 +199,12 @@ def adjust_scores(scores, seen=None, penalties=None, bias=None, mask=None, out=N
         penalties = _tensor(penalties, "penalties", T.f32, 2).contiguous()
         if off.shape[0] != nq + 1 or penalties.shape != (nq, 3):
             raise _bad("offsets must be [nq + 1] and penalties [nq, 3]")
-        if ids.numel() == 0:
+        nids = ids.numel()
+        if nids == 0:
             off = ids = penalties = None
     bias, bstride = _bias_arg(bias, nq, n, True)
     mask, mstride = _mask_arg(mask, nq, n)
-    _call(T.lib.ndbhip_scores_adjust_device, _p(src), T.types[src.dtype], nq, n, stride, _p(off), _p(ids), _p(penalties), _p(bias), bstride,
+    _call(T.lib.ndbhip_scores_adjust_device, _p(src), T.types[src.dtype], nq, n, stride, _p(off), _p(ids), nids, _p(penalties), _p(bias), bstride,
           _p(mask), mstride, _p(out), ostride)
     return out
 

@@ -357,6 +357,18 @@ def test_search_scales_of_zero_and_infinite_products():
                 same(sc, best(s, k)[1])
 
 
+@pytest.mark.parametrize("nq,n,k", [(1, 500, 7), (40, 3000, 300), (300, 60_000, 20)])
+def test_search_takes_minus_zero_and_zero_for_equal(nq, n, k):
+    c = torch.zeros(n, 32, dtype=torch.int8)
+    s = torch.ones(n)
+    s[::2] = -1.0
+    t = nd.Int8Table(32)
+    t.load(c.cuda(), s.cuda())
+    ids, sc = t.search(torch.ones(nq, 32, device="cuda"), k)
+    same(ids, torch.arange(k)[None].repeat(nq, 1))
+    assert not sc.any() and not torch.signbit(sc).any()
+
+
 def test_search_of_an_empty_table_and_of_no_queries():
     t = nd.Int8Table(8)
     ids, sc = t.search(torch.ones(3, 8, device="cuda"), 4)
@@ -476,6 +488,19 @@ def test_adjust_strides(dtype):
     assert bool((wide[:, :5] == 3).all()) and bool((wide[:, 338:] == 3).all())
 
 
+def test_adjust_offsets_outside_the_ids():
+    """offsets that run out of the list, or backwards, count what there is"""
+    s = rand(1, 4, 50)
+    ids = torch.tensor([1, 2, 2, 3], dtype=torch.int32)
+    pen = torch.tensor([[2.0, 0.5, 0.25]]).repeat(4, 1)
+    off = torch.tensor([-7, 2, 1, 1 << 40, 5])
+    got = nd.adjust_scores(s.cuda(), (off.cuda(), ids.cuda()), pen.cuda())
+    same(got[:1], adjust(s[:1], torch.tensor([0, 2]), ids, pen, None, None))
+    same(got[1:2], s[1:2])
+    same(got[2:3], adjust(s[2:3], torch.tensor([1, 4]), ids, pen, None, None))
+    same(got[3:], s[3:])
+
+
 # ------------------------------------------------------------------ together, streams, graphs
 
 def test_scores_adjusted_and_ranked_are_the_search():
@@ -569,6 +594,32 @@ def test_streams_of_torch_and_of_the_library():
     cur = C.c_void_p()
     _lib.check(_lib.lib().ndbhip_swap_thread_stream(None, C.byref(cur)))
     assert not cur.value
+
+
+def test_two_threads_search_one_table_at_the_same_time():
+    import threading
+    n, dim = 50_000, 128
+    t = nd.Int8Table(dim)
+    t.load(rand(1, n, dim).cuda())
+    qs = [rand(2, 300, dim).cuda(), rand(3, 7, dim).cuda()]
+    refs = [t.search(q, 20) for q in qs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    ids, sc = t.search(qs[i], 20)
+                    if not (torch.equal(ids, refs[i][0]) and torch.equal(sc, refs[i][1])):
+                        bad.append(i)
+        except Exception as e:          # noqa: BLE001 (reported below)
+            bad.append(e)
+
+    th = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [x.start() for x in th]
+    [x.join() for x in th]
+    assert not bad
 
 
 def test_results_do_not_change_from_call_to_call():

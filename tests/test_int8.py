@@ -95,14 +95,15 @@ def test_product_and_search_arguments():
 
 @no_gpu
 def test_adjust_arguments():
-    good = [P, 0, 4, 70, 70, P, P, P, P, 0, P, 3, 2 * P, 70]
+    good = [P, 0, 4, 70, 70, P, P, 5, P, P, 0, P, 3, 2 * P, 70]
     assert L.ndbhip_scores_adjust_device(*good) == NODEVICE
-    for at, v in ((0, None), (1, 3), (2, -1), (3, -1), (4, 69), (6, None), (7, None), (9, 69), (9, -1), (11, 2), (11, -1), (12, None), (13, 69)):
+    for at, v in ((0, None), (1, 3), (2, -1), (3, -1), (4, 69), (6, None), (7, -1), (8, None), (10, 69), (10, -1), (12, 2),
+                  (12, -1), (13, None), (14, 69)):
         a = list(good)
         a[at] = v
         assert L.ndbhip_scores_adjust_device(*a) == INVALID, (at, v)
-    assert L.ndbhip_scores_adjust_device(P, 0, 4, 70, 70, None, None, None, None, 0, None, 0, P, 71) == INVALID     # in place, another stride
-    assert L.ndbhip_scores_adjust_device(P, 0, 4, 70, 70, None, None, None, None, 0, None, 0, P, 70) == NODEVICE
+    assert L.ndbhip_scores_adjust_device(P, 0, 4, 70, 70, None, None, 0, None, None, 0, None, 0, P, 71) == INVALID     # in place, another stride
+    assert L.ndbhip_scores_adjust_device(P, 0, 4, 70, 70, None, None, 0, None, None, 0, None, 0, P, 70) == NODEVICE
 
 
 def test_errors_have_a_text():
