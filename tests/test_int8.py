@@ -4,6 +4,8 @@ import ctypes as C
 import importlib.util
 import os
 import random
+import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -112,6 +114,31 @@ def test_errors_have_a_text():
     assert "dim" in _lib.last_error()
     with pytest.raises(_lib.NdbHipError):
         _lib.check(INVALID)
+
+
+# ------------------------------------------------------------------ the generated code
+
+@pytest.mark.skipif(not os.path.exists("/opt/rocm/bin/hipcc"), reason="needs hipcc")
+def test_generated_code_of_the_8_bit_kernels(tmp_path):
+    """M0, which the LDS copies write in inline assembly, is nobody else's; nothing spills to scratch; no packed fp32"""
+    src = os.path.join(ROOT, "neurondb_amd", "csrc", "ndbhip_int8.hip")
+    make = open(os.path.join(os.path.dirname(src), "Makefile")).read()
+    flags = re.search(r"^CXXFLAGS \?= (.*?[^\\])$", make, re.S | re.M).group(1).replace("\\\n", " ").replace("$(ARCH)", "gfx950").split()
+    flags += re.search(r"ndbhip_int8.o: CXXFLAGS \+= (.*)", make).group(1).split()
+    out = str(tmp_path / "i8.s")
+    subprocess.run(["/opt/rocm/bin/hipcc", *flags, "--cuda-device-only", "-S", src, "-o", out], check=True, stderr=subprocess.DEVNULL)
+    s = open(out).read()
+    lines = s.splitlines()
+    m0 = [i for i, l in enumerate(lines) if re.search(r"\bm0\b", l.split(";")[0])]
+    assert len(m0) > 50
+    for i in m0:
+        assert re.match(r"\ts_mov_b32 m0, s\d+", lines[i]) and "s_nop 4" in lines[i + 1] and "global_load_lds_dword" in lines[i + 2], lines[i]
+    assert len([l for l in lines if "global_load_lds" in l]) == len(m0)
+    assert set(re.findall(r"\.amdhsa_private_segment_fixed_size (\d+)", s)) == {"0"}
+    assert not re.search(r"v_pk_\w+_f32", s)
+    tiles = [k for k in re.findall(r"\.amdhsa_kernel (\S+)", s) if "k_i8_tile" in k]
+    assert len(tiles) == 2 * (4 + 2 * 3)
+    assert s.count("v_mfma_i32_32x32x32_i8") >= 32 * len(tiles)
 
 
 # ------------------------------------------------------------------ the plain forms of perf/operators.py, on the CPU
