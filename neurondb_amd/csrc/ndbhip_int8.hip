@@ -331,13 +331,41 @@ i8_score(int dot, float rs, float qs)
 	return ((float) dot * rs) * qs;
 }
 
+/* a score or two; PAST: past the caches */
+template <bool PAST, class V>
+__device__ __forceinline__ void
+i8_store(void *p, const V &v)
+{
+	if constexpr (sizeof(V) == 4)
+	{
+		typedef uint32_t word __attribute__((aligned(2)));
+		uint32_t	w;
+
+		__builtin_memcpy(&w, &v, 4);
+		if (PAST)
+			__builtin_nontemporal_store(w, (word *) p);
+		else
+			*(word *) p = w;
+	}
+	else
+	{
+		uint16_t	w;
+
+		__builtin_memcpy(&w, &v, 2);
+		if (PAST)
+			__builtin_nontemporal_store(w, (uint16_t *) p);
+		else
+			*(uint16_t *) p = w;
+	}
+}
+
 /*
  * Writes the block of sums of row block rb and the query block that starts at query q0.  The matrix instruction had the
  * queries as its first operand: lane l has row l % 32 and, in register 4 g + j, query 8 g + 4 (l / 32) + j, so that a store
  * covers 32 neighbouring scores of each of two queries, whatever the matrix's alignment.  rs, bias: of the lane's row;
  * qs: the block's 32 query scales, in LDS.
  */
-template <bool BIAS, class T>
+template <bool BIAS, bool PAST, class T>
 __device__ __forceinline__ void
 i8_write_scores(const I8Out &o, float rs, float bias, const float *qs, uint32_t rb, uint32_t q0, const i8_v16i &acc)
 {
@@ -360,17 +388,35 @@ i8_write_scores(const I8Out &o, float rs, float bias, const float *qs, uint32_t 
 				s[4 * g4 + j] = s[4 * g4 + j] + bias;
 		}
 	}
+	if constexpr (sizeof(T) == 2)
+		if (q0 + 32 <= o.nq && rb * 32 + 32 <= o.n)
+		{
+			/* 16 bits: two lanes trade a score, so that each stores two neighbouring ones of one query */
+			const bool	odd = lane & 1;
+			T		   *pair = out + (odd ? o.ostride - 1 : 0);
+
+#pragma unroll
+			for (int i = 0; i < 16; i += 2)
+			{
+				const float got = __uint_as_float((uint32_t) __builtin_amdgcn_mov_dpp((int) __float_as_uint(odd ? s[i] : s[i + 1]), 0xB1, 0xF, 0xF, true));
+				I8Vec<T, 2> v;
+
+				v.v[0] = I8Elem<T>::store(odd ? got : s[i]);
+				v.v[1] = I8Elem<T>::store(odd ? s[i + 1] : got);
+				i8_store<PAST>(pair + (int64_t) (8 * (i / 4) + i % 4) * o.ostride, v);
+			}
+			return;
+		}
 	if (r >= o.n)
 		return;
-	if (q0 + 32 <= o.nq)
 #pragma unroll
-		for (int i = 0; i < 16; i++)
-			out[(int64_t) (8 * (i / 4) + i % 4) * o.ostride] = I8Elem<T>::store(s[i]);
-	else
-#pragma unroll
-		for (int i = 0; i < 16; i++)
-			if (qh + 8 * (i / 4) + i % 4 < o.nq)
-				out[(int64_t) (8 * (i / 4) + i % 4) * o.ostride] = I8Elem<T>::store(s[i]);
+	for (int i = 0; i < 16; i++)
+		if (q0 + 32 <= o.nq || qh + 8 * (i / 4) + i % 4 < o.nq)
+		{
+			const I8Vec<T, 1> v = {{I8Elem<T>::store(s[i])}};
+
+			i8_store<PAST>(out + (int64_t) (8 * (i / 4) + i % 4) * o.ostride, v);
+		}
 }
 
 /*
@@ -449,7 +495,7 @@ i8_mask_word(const I8Out &o, uint32_t rb, uint32_t q)
 /* what an instance of the product kernels does with its sums */
 template <int MODE_, bool BIAS_, bool MASK_, class T_> struct I8Kind
 {
-	static constexpr int MODE = MODE_;		/* 0 writes scores, 1 leaves maxima */
+	static constexpr int MODE = MODE_;		/* 0 writes scores, 2 the same past the caches, 1 leaves maxima */
 	static constexpr bool BIAS = BIAS_, MASK = MASK_;
 	typedef T_	T;
 };
@@ -465,7 +511,7 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 {
 	constexpr int U = TB == 1 ? 8 : 4;
 	__shared__ __attribute__((aligned(16))) float s_m[KIND::MODE == 1 ? TB * 32 : 1][4];
-	__shared__ __attribute__((aligned(16))) float s_rs[4][32], s_bias[KIND::BIAS ? 4 : 1][32], s_qs[4][KIND::MODE == 0 ? TB * 32 : 1];
+	__shared__ __attribute__((aligned(16))) float s_rs[4][32], s_bias[KIND::BIAS ? 4 : 1][32], s_qs[4][KIND::MODE != 1 ? TB * 32 : 1];
 	const int	lane = threadIdx.x & 63;
 	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const uint32_t rb = min(blockIdx.x * 4 + wave, nrb - 1);	/* (waves behind the last block do it over) */
@@ -508,7 +554,7 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 			if (k + u * 32 < kp)
 #pragma unroll
 				for (int t = 0; t < TB; t++)
-					acc[t] = KIND::MODE == 0 ? __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[u][t], av[u], acc[t], 0, 0, 0) :
+					acc[t] = KIND::MODE != 1 ? __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[u][t], av[u], acc[t], 0, 0, 0) :
 						__builtin_amdgcn_mfma_i32_32x32x32_i8(av[u], bv[u][t], acc[t], 0, 0, 0);
 	}
 	/* (a wave's own LDS: what it writes it reads in order) */
@@ -517,7 +563,7 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 		s_rs[wave][lane] = my_rs;
 		if (KIND::BIAS)
 			s_bias[wave][lane] = my_bias;
-		if (KIND::MODE == 0)
+		if (KIND::MODE != 1)
 #pragma unroll
 			for (int t = 0; t < TB; t++)
 				s_qs[wave][t * 32 + lane] = qs[t];
@@ -526,8 +572,8 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 #pragma unroll
 	for (int t = 0; t < TB; t++)
 	{
-		if (KIND::MODE == 0)
-			i8_write_scores<KIND::BIAS, typename KIND::T>(o, my_rs, my_bias, s_qs[wave] + t * 32, rb, (qb0 + t) * 32, acc[t]);
+		if (KIND::MODE != 1)
+			i8_write_scores<KIND::BIAS, KIND::MODE == 2, typename KIND::T>(o, my_rs, my_bias, s_qs[wave] + t * 32, rb, (qb0 + t) * 32, acc[t]);
 		else
 		{
 			const float m = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs[wave], s_bias[KIND::BIAS ? wave : 0], bits[t], qs[t], acc[t]);
@@ -749,7 +795,7 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 
 	uint32_t	buf = 0, slot = 0;
 	auto		mul = [](const i8_v4i &r, const i8_v4i &q, const i8_v16i &c) -> i8_v16i {
-		return KIND::MODE == 0 ? __builtin_amdgcn_mfma_i32_32x32x32_i8(q, r, c, 0, 0, 0) :
+		return KIND::MODE != 1 ? __builtin_amdgcn_mfma_i32_32x32x32_i8(q, r, c, 0, 0, 0) :
 			__builtin_amdgcn_mfma_i32_32x32x32_i8(r, q, c, 0, 0, 0);
 	};
 
@@ -801,11 +847,11 @@ k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restric
 #pragma unroll
 		for (int t = 0; t < WQ; t++)
 		{
-			if (KIND::MODE == 0)
+			if (KIND::MODE != 1)
 			{
 #pragma unroll
 				for (int i = 0; i < 4; i++)
-					i8_write_scores<KIND::BIAS, typename KIND::T>(o, s_rs[slot][(wr * 4 + i) * 32 + (lane & 31)],
+					i8_write_scores<KIND::BIAS, KIND::MODE == 2, typename KIND::T>(o, s_rs[slot][(wr * 4 + i) * 32 + (lane & 31)],
 																  s_bias[KIND::BIAS ? slot : 0][(wr * 4 + i) * 32 + (lane & 31)],
 																  s_qs[slot] + (wq * WQ + t) * 32, rb0 + i, (qb0 + t) * 32, acc[i][t]);
 			}
@@ -1911,6 +1957,14 @@ template <class T>
 static int
 i8_multiply_scores(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
 {
+	/*
+	 * Scores that fill the last level cache push the operands out of the L2s on their way: stored past the caches, 1024 x 131072
+	 * takes 172 -> 128 us at 768 dimensions and 247 -> 205 at 1536 (fp32; bf16 171 -> 139, 248 -> 208).  Smaller
+	 * matrices and short rows lose by it (256 x 131072 x 768 42 -> 45, 768 x 131072 x 256 83 -> 90).
+	 */
+	if ((uint64_t) o.nq * o.n * sizeof(T) > ((uint64_t) 192 << 20) && t->kp >= 512)
+		return o.bias ? i8_multiply_kind<I8Kind<2, true, false, T>>(t, queries, o) :
+			i8_multiply_kind<I8Kind<2, false, false, T>>(t, queries, o);
 	return o.bias ? i8_multiply_kind<I8Kind<0, true, false, T>>(t, queries, o) : i8_multiply_kind<I8Kind<0, false, false, T>>(t, queries, o);
 }
 

@@ -248,6 +248,24 @@ def test_non_finite_rows_and_queries():
     assert bool((ids[1] == -1).all()) and int((ids[0] == -1).sum()) == 2
 
 
+@pytest.mark.parametrize("nq,n,dim", [(130, 400_003, 520), (31, 1_700_001, 513), (260, 400_003, 520)])
+@pytest.mark.parametrize("out_t", [F32, BF16])
+def test_scores_that_no_cache_holds(nq, n, dim, out_t):
+    """large matrices are stored another way: the same scores as in pieces, and nothing beside them"""
+    t = nd.Int8Table(dim)
+    t.load(torch.randn(n, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(n)))
+    q, bias = rand(nq, nq, dim).cuda(), rand(3, n).cuda()
+    out = torch.full((nq, n + 5), 9.0, dtype=out_t, device="cuda")
+    t.scores(q, bias=bias, out=out[:, 2:2 + n])
+    for at in range(0, nq, 13):
+        same(out[at:at + 13, 2:2 + n], t.scores(q[at:at + 13], bias=bias, dtype=out_t))
+    assert bool((out[:, :2] == 9).all()) and bool((out[:, 2 + n:] == 9).all())
+    codes, scales = t.export()
+    rows = torch.tensor([0, 77, n // 2, n - 1])
+    ref = scores_of(*quantise(q), codes[rows.cuda()].cpu(), scales[rows.cuda()].cpu(), bias[rows.cuda()].cpu())
+    same(out[:, 2:2 + n][:, rows.cuda()], ref.to(out_t))
+
+
 def test_more_scores_than_32_bits_count():
     n, nq, dim = 1_000_000, 2200, 16
     rows, q = torch.randn(n, dim, device="cuda"), torch.randn(nq, dim, device="cuda")

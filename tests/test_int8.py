@@ -137,7 +137,7 @@ def test_generated_code_of_the_8_bit_kernels(tmp_path):
     assert set(re.findall(r"\.amdhsa_private_segment_fixed_size (\d+)", s)) == {"0"}
     assert not re.search(r"v_pk_\w+_f32", s)
     tiles = [k for k in re.findall(r"\.amdhsa_kernel (\S+)", s) if "k_i8_tile" in k]
-    assert len(tiles) == 2 * (4 + 2 * 3)
+    assert len(tiles) == 2 * (4 + 2 * 2 * 3)
     assert s.count("v_mfma_i32_32x32x32_i8") >= 32 * len(tiles)
 
 
