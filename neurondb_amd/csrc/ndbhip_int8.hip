@@ -501,49 +501,65 @@ template <int MODE_, bool BIAS_, bool MASK_, class T_> struct I8Kind
 };
 
 /*
- * Few queries: a wave multiplies one block of 32 rows with TB blocks of 32 queries straight from memory, U steps of 32
+ * Few queries: a wave multiplies RW blocks of 32 rows with TB blocks of 32 queries straight from memory, U steps of 32
  * dimensions requested at a time; the queries stay in the caches.  What the sums are combined with is requested first.
- * Bound by HBM: the table is read once for every TB * 32 queries.
+ * Bound by HBM: the table is read once for every TB * 32 queries (one query, 1M x 768: 125 us, 6.1 TB/s).
  */
-template <int TB, class KIND>
+template <int RW, int TB, class KIND>
 __global__ __launch_bounds__(256) void
 k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrb, I8Out o)
 {
 	constexpr int U = TB == 1 ? 8 : 4;
-	__shared__ __attribute__((aligned(16))) float s_m[KIND::MODE == 1 ? TB * 32 : 1][4];
-	__shared__ __attribute__((aligned(16))) float s_rs[4][32], s_bias[KIND::BIAS ? 4 : 1][32], s_qs[4][KIND::MODE != 1 ? TB * 32 : 1];
+	__shared__ __attribute__((aligned(16))) float s_m[KIND::MODE == 1 ? TB * 32 : 1][4 * RW];
+	__shared__ __attribute__((aligned(16))) float s_rs[4 * RW][32], s_bias[KIND::BIAS ? 4 * RW : 1][32];
+	__shared__ __attribute__((aligned(16))) float s_qs[4][KIND::MODE != 1 ? TB * 32 : 1];
 	const int	lane = threadIdx.x & 63;
 	const int	wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const uint32_t rb = min(blockIdx.x * 4 + wave, nrb - 1);	/* (waves behind the last block do it over) */
 	const uint32_t qb0 = blockIdx.y * TB;
-	const unsigned char *a = rows + (size_t) rb * 32u * kp + lane * 16;
 	const unsigned char *b = queries + (size_t) qb0 * 32u * kp + lane * 16;
-	const uint32_t row = rb * 32 + (lane & 31);
-	const float my_rs = o.rscale[row];
-	const float my_bias = KIND::BIAS && row < o.n ? o.bias[row] : 0.0f;
-	float		qs[TB];
-	uint32_t	bits[TB];
-	i8_v16i		acc[TB];
+	const unsigned char *a[RW];
+	uint32_t	rb[RW];
+	float		my_rs[RW], my_bias[RW], qs[TB];
+	uint32_t	bits[RW][TB];
+	i8_v16i		acc[RW][TB];
 
+#pragma unroll
+	for (int i = 0; i < RW; i++)
+	{
+		/* (waves behind the last block do it over) */
+		rb[i] = min((blockIdx.x * 4 + wave) * RW + i, nrb - 1);
+		a[i] = rows + (size_t) rb[i] * 32u * kp + lane * 16;
+
+		const uint32_t row = rb[i] * 32 + (lane & 31);
+
+		my_rs[i] = o.rscale[row];
+		my_bias[i] = KIND::BIAS && row < o.n ? o.bias[row] : 0.0f;
+	}
 #pragma unroll
 	for (int t = 0; t < TB; t++)
 	{
 		const uint32_t q = (qb0 + t) * 32 + (lane & 31);
 
 		qs[t] = q < o.nq ? o.qscale[q] : 1.0f;
-		bits[t] = KIND::MASK ? i8_mask_word(o, rb, q) : 0u;
 #pragma unroll
-		for (int i = 0; i < 16; i++)
-			acc[t][i] = 0;
+		for (int i = 0; i < RW; i++)
+		{
+			bits[i][t] = KIND::MASK ? i8_mask_word(o, rb[i], q) : 0u;
+#pragma unroll
+			for (int e = 0; e < 16; e++)
+				acc[i][t][e] = 0;
+		}
 	}
 	for (uint32_t k = 0; k < kp; k += 32 * U)
 	{
-		i8_v4i		av[U], bv[U][TB];
+		i8_v4i		av[U][RW], bv[U][TB];
 
 		/* (a step behind the last one asks for that one again and is not multiplied) */
 #pragma unroll
 		for (int u = 0; u < U; u++)
-			av[u] = *(const i8_v4i *) (a + (size_t) min(k + u * 32, kp - 32) * 32);
+#pragma unroll
+			for (int i = 0; i < RW; i++)
+				av[u][i] = *(const i8_v4i *) (a[i] + (size_t) min(k + u * 32, kp - 32) * 32);
 #pragma unroll
 		for (int u = 0; u < U; u++)
 #pragma unroll
@@ -553,16 +569,22 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 		for (int u = 0; u < U; u++)
 			if (k + u * 32 < kp)
 #pragma unroll
-				for (int t = 0; t < TB; t++)
-					acc[t] = KIND::MODE != 1 ? __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[u][t], av[u], acc[t], 0, 0, 0) :
-						__builtin_amdgcn_mfma_i32_32x32x32_i8(av[u], bv[u][t], acc[t], 0, 0, 0);
+				for (int i = 0; i < RW; i++)
+#pragma unroll
+					for (int t = 0; t < TB; t++)
+						acc[i][t] = KIND::MODE != 1 ? __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[u][t], av[u][i], acc[i][t], 0, 0, 0) :
+							__builtin_amdgcn_mfma_i32_32x32x32_i8(av[u][i], bv[u][t], acc[i][t], 0, 0, 0);
 	}
 	/* (a wave's own LDS: what it writes it reads in order) */
 	if (lane < 32)
 	{
-		s_rs[wave][lane] = my_rs;
-		if (KIND::BIAS)
-			s_bias[wave][lane] = my_bias;
+#pragma unroll
+		for (int i = 0; i < RW; i++)
+		{
+			s_rs[wave * RW + i][lane] = my_rs[i];
+			if (KIND::BIAS)
+				s_bias[wave * RW + i][lane] = my_bias[i];
+		}
 		if (KIND::MODE != 1)
 #pragma unroll
 			for (int t = 0; t < TB; t++)
@@ -571,30 +593,32 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 	__builtin_amdgcn_wave_barrier();
 #pragma unroll
 	for (int t = 0; t < TB; t++)
-	{
-		if (KIND::MODE != 1)
-			i8_write_scores<KIND::BIAS, KIND::MODE == 2, typename KIND::T>(o, my_rs, my_bias, s_qs[wave] + t * 32, rb, (qb0 + t) * 32, acc[t]);
-		else
-		{
-			const float m = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs[wave], s_bias[KIND::BIAS ? wave : 0], bits[t], qs[t], acc[t]);
+#pragma unroll
+		for (int i = 0; i < RW; i++)
+			if (KIND::MODE != 1)
+				i8_write_scores<KIND::BIAS, KIND::MODE == 2, typename KIND::T>(o, my_rs[i], my_bias[i], s_qs[wave] + t * 32, rb[i],
+																			   (qb0 + t) * 32, acc[i][t]);
+			else
+			{
+				const float m = i8_block_max<KIND::BIAS, KIND::MASK>(s_rs[wave * RW + i], s_bias[KIND::BIAS ? wave * RW + i : 0], bits[i][t],
+																	 qs[t], acc[i][t]);
 
-			if (lane < 32)
-				s_m[t * 32 + lane][wave] = m;
-		}
-	}
+				if (lane < 32)
+					s_m[t * 32 + lane][wave * RW + i] = m;
+			}
 	if (KIND::MODE == 1)
 	{
 		__syncthreads();
-		for (int i = threadIdx.x; i < TB * 32; i += 256)
+		for (int e = threadIdx.x; e < TB * 32 * RW; e += 256)
 		{
-			const uint32_t q = qb0 * 32 + i;
+			const uint32_t q = qb0 * 32 + e / RW, quad = blockIdx.x * RW + e % RW;
 
-			if (q < o.nq)
+			if (q < o.nq && quad * 4 < o.ngp)
 			{
-				const float4 m = *(const float4 *) s_m[i];
+				const float4 m = *(const float4 *) &s_m[e / RW][e % RW * 4];
 
-				*(float4 *) (o.gmax + (size_t) q * o.ngp + blockIdx.x * 4) = m;
-				o.qmax[(size_t) q * (o.ngp / 4) + blockIdx.x] = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+				*(float4 *) (o.gmax + (size_t) q * o.ngp + quad * 4) = m;
+				o.qmax[(size_t) q * (o.ngp / 4) + quad] = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
 			}
 		}
 	}
@@ -1939,10 +1963,15 @@ i8_multiply_kind(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &
 	 */
 	if (o.nq <= 64 || nrt * w128 * (t->kp + 128) <= 80000)
 	{
+		/* (two query blocks: with two row blocks a wave the queries are read half as often, from 64 k rows on: 50 x 300007 x 1536
+		 * 108 -> 96 us, 40 x 32000 x 768 9.8 -> 11.1) */
 		if (nqb == 1)
-			hipLaunchKernelGGL((k_i8_stream<1, KIND>), dim3((nrb + 3) / 4), dim3(256), 0, g.stream, t->d_codes, queries, t->kp, nrb, o);
+			hipLaunchKernelGGL((k_i8_stream<1, 1, KIND>), dim3((nrb + 3) / 4), dim3(256), 0, g.stream, t->d_codes, queries, t->kp, nrb, o);
+		else if (nrb >= 2048)
+			hipLaunchKernelGGL((k_i8_stream<2, 2, KIND>), dim3((nrb + 7) / 8, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
+							   nrb, o);
 		else
-			hipLaunchKernelGGL((k_i8_stream<2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
+			hipLaunchKernelGGL((k_i8_stream<1, 2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
 							   nrb, o);
 	}
 	else if (nrt * w256 >= (uint32_t) g.num_cus && 10 * w256 * 2 <= 12 * w128)
