@@ -495,7 +495,7 @@ i8_mask_word(const I8Out &o, uint32_t rb, uint32_t q)
 /* what an instance of the product kernels does with its sums */
 template <int MODE_, bool BIAS_, bool MASK_, class T_> struct I8Kind
 {
-	static constexpr int MODE = MODE_;		/* 0 writes scores, 2 the same past the caches, 1 leaves maxima */
+	static constexpr int MODE = MODE_;		/* 0 writes scores, 1 leaves maxima, 2 writes scores past the caches (tiles only) */
 	static constexpr bool BIAS = BIAS_, MASK = MASK_;
 	typedef T_	T;
 };
@@ -596,7 +596,7 @@ k_i8_stream(const unsigned char *__restrict__ rows, const unsigned char *__restr
 #pragma unroll
 		for (int i = 0; i < RW; i++)
 			if (KIND::MODE != 1)
-				i8_write_scores<KIND::BIAS, KIND::MODE == 2, typename KIND::T>(o, my_rs[i], my_bias[i], s_qs[wave] + t * 32, rb[i],
+				i8_write_scores<KIND::BIAS, false, typename KIND::T>(o, my_rs[i], my_bias[i], s_qs[wave] + t * 32, rb[i],
 																			   (qb0 + t) * 32, acc[i][t]);
 			else
 			{
@@ -1948,36 +1948,47 @@ i8_tile_launch(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
 }
 
 template <class KIND>
+static void
+i8_stream_launch(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
+{
+	const uint32_t nrb = (o.n + 31) / 32, nqb = (o.nq + 31) / 32;
+
+	/* two query blocks: with two row blocks a wave the queries are read half as often, which pays from 64 k rows on (50 x 300007 x
+	 * 1536 108 -> 96 us, 40 x 32000 x 768 9.8 -> 11.1) */
+	if (nqb == 1)
+		hipLaunchKernelGGL((k_i8_stream<1, 1, KIND>), dim3((nrb + 3) / 4), dim3(256), 0, g.stream, t->d_codes, queries, t->kp, nrb, o);
+	else if (nrb >= 2048)
+		hipLaunchKernelGGL((k_i8_stream<2, 2, KIND>), dim3((nrb + 7) / 8, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
+						   nrb, o);
+	else
+		hipLaunchKernelGGL((k_i8_stream<1, 2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
+						   nrb, o);
+}
+
+/*
+ * Up to 64 queries the table's bytes are what counts, and the stream reads them as fast as memory gives them.  Above, a tile pays
+ * where there are enough of them to cover its start (scores of fp16; stream / 128-query tile / 256-query tile in us): 96 x
+ * 16000 x 768 10.6 / 11.0 / 14.2, 256 x 16000 x 768 14.9 / 12.4 / 15.0, 96 x 64000 x 64 7.5 / 8.6 / 9.7, 256 x 64000 x 64 11.9 / 11.3
+ * / 11.2.  The wide tile does a fifth more per query of its width (512 x 256000 x 768: 257 / 163 / 133) but wants a tile for
+ * every compute unit (512 x 16000 x 768: 20.2 / 14.5 / 17.1).  What goes past the caches is always many tiles.
+ */
+template <class KIND>
 static int
 i8_multiply_kind(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
 {
-	const uint32_t nrb = (o.n + 31) / 32, nqb = (o.nq + 31) / 32;
 	const uint64_t nrt = (o.n + 255) / 256, w128 = (o.nq + 127) / 128, w256 = (o.nq + 255) / 256;
+	bool		few = false;
 
-	/*
-	 * Up to 64 queries the table's bytes are what counts, and the stream reads them as fast as memory gives them.  Above, a
-	 * tile pays where there are enough of them to cover its start (scores of fp16; stream / 128-query tile / 256-query tile in
-	 * us): 96 x 16000 x 768 10.6 / 11.0 / 14.2, 256 x 16000 x 768 14.9 / 12.4 / 15.0, 96 x 64000 x 64 7.5 / 8.6 / 9.7, 256 x 64000
-	 * x 64 11.9 / 11.3 / 11.2.  The wide tile does a fifth more per query of its width (512 x 256000 x 768: 257 / 163 / 133) but
-	 * wants a tile for every compute unit (512 x 16000 x 768: 20.2 / 14.5 / 17.1).
-	 */
-	if (o.nq <= 64 || nrt * w128 * (t->kp + 128) <= 80000)
+	if constexpr (KIND::MODE != 2)
+		if ((few = o.nq <= 64 || nrt * w128 * (t->kp + 128) <= 80000))
+			i8_stream_launch<KIND>(t, queries, o);
+	if (!few)
 	{
-		/* (two query blocks: with two row blocks a wave the queries are read half as often, from 64 k rows on: 50 x 300007 x 1536
-		 * 108 -> 96 us, 40 x 32000 x 768 9.8 -> 11.1) */
-		if (nqb == 1)
-			hipLaunchKernelGGL((k_i8_stream<1, 1, KIND>), dim3((nrb + 3) / 4), dim3(256), 0, g.stream, t->d_codes, queries, t->kp, nrb, o);
-		else if (nrb >= 2048)
-			hipLaunchKernelGGL((k_i8_stream<2, 2, KIND>), dim3((nrb + 7) / 8, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
-							   nrb, o);
+		if (nrt * w256 >= (uint32_t) g.num_cus && 10 * w256 * 2 <= 12 * w128)
+			i8_tile_launch<4, KIND>(t, queries, o);
 		else
-			hipLaunchKernelGGL((k_i8_stream<1, 2, KIND>), dim3((nrb + 3) / 4, (nqb + 1) / 2), dim3(256), 0, g.stream, t->d_codes, queries, t->kp,
-							   nrb, o);
+			i8_tile_launch<2, KIND>(t, queries, o);
 	}
-	else if (nrt * w256 >= (uint32_t) g.num_cus && 10 * w256 * 2 <= 12 * w128)
-		i8_tile_launch<4, KIND>(t, queries, o);
-	else
-		i8_tile_launch<2, KIND>(t, queries, o);
 	HIP_TRY(hipGetLastError());
 	return NDBHIP_OK;
 }
@@ -1987,11 +1998,13 @@ static int
 i8_multiply_scores(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
 {
 	/*
-	 * Scores that fill the last level cache push the operands out of the L2s on their way: stored past the caches, 1024 x 131072
-	 * takes 172 -> 128 us at 768 dimensions and 247 -> 205 at 1536 (fp32; bf16 171 -> 139, 248 -> 208).  Smaller
-	 * matrices and short rows lose by it (256 x 131072 x 768 42 -> 45, 768 x 131072 x 256 83 -> 90).
+	 * Scores that fill the last level cache (256 MB) push the table out of it.  Stored past the caches they leave it there for the
+	 * next batch: back to back, 1024 x 131072 takes 155 -> 125 us at 512 dimensions, 186 -> 150 at 768 and 267 -> 231 at 1536
+	 * (fp32; bf16 258 -> 222).  Where nothing is kept it costs a little (three tables in turn 267 -> 277; a table larger than
+	 * the cache, 512 x 400000 x 1536 bf16: 362 -> 385), and smaller matrices or short rows lose by it (256 x 131072 x 768
+	 * 42 -> 45, 768 x 131072 x 256 83 -> 90).
 	 */
-	if ((uint64_t) o.nq * o.n * sizeof(T) > ((uint64_t) 192 << 20) && t->kp >= 512)
+	if ((uint64_t) o.nq * o.n * sizeof(T) > ((uint64_t) 192 << 20) && t->kp >= 512 && (uint64_t) t->np * t->kp <= ((uint64_t) 256 << 20))
 		return o.bias ? i8_multiply_kind<I8Kind<2, true, false, T>>(t, queries, o) :
 			i8_multiply_kind<I8Kind<2, false, false, T>>(t, queries, o);
 	return o.bias ? i8_multiply_kind<I8Kind<0, true, false, T>>(t, queries, o) : i8_multiply_kind<I8Kind<0, false, false, T>>(t, queries, o);

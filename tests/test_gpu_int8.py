@@ -248,7 +248,7 @@ def test_non_finite_rows_and_queries():
     assert bool((ids[1] == -1).all()) and int((ids[0] == -1).sum()) == 2
 
 
-@pytest.mark.parametrize("nq,n,dim", [(130, 400_003, 520), (31, 1_700_001, 513), (260, 400_003, 520)])
+@pytest.mark.parametrize("nq,n,dim", [(130, 400_003, 520), (31, 1_700_001, 513), (280, 400_003, 520), (1000, 60_001, 1000)])
 @pytest.mark.parametrize("out_t", [F32, BF16])
 def test_scores_that_no_cache_holds(nq, n, dim, out_t):
     """large matrices are stored another way: the same scores as in pieces, and nothing beside them"""
