@@ -2220,16 +2220,17 @@ scores_adjust_launch(const void *s, int64_t stride, int nq, int64_t n, const int
 	constexpr int VEC = 16 / sizeof(T);
 	const int	u = (int64_t) nq * n >= ((int64_t) 4 << 20) ? 4 : 2, cols = 256 * VEC * u;
 
-	for (int q0 = 0; q0 < nq; q0 += 65535)
+	/* (64 bits: behind 2^31 - 65536 queries the next start is not an int) */
+	for (int64_t q0 = 0; q0 < nq; q0 += 65535)
 	{
-		const dim3	grid((unsigned) ((n + cols - 1) / cols), std::min(65535, nq - q0));
+		const dim3	grid((unsigned) ((n + cols - 1) / cols), (unsigned) std::min<int64_t>(65535, nq - q0));
 
 		if (u == 4)
 			hipLaunchKernelGGL((k_scores_adjust<T, 4>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, off, ids, nids, pen, bias,
-							   bias_stride, mask, mask_stride, (T *) out, ostride, q0);
+							   bias_stride, mask, mask_stride, (T *) out, ostride, (int) q0);
 		else
 			hipLaunchKernelGGL((k_scores_adjust<T, 2>), grid, dim3(256), 0, g.stream, (const T *) s, stride, n, off, ids, nids, pen, bias,
-							   bias_stride, mask, mask_stride, (T *) out, ostride, q0);
+							   bias_stride, mask, mask_stride, (T *) out, ostride, (int) q0);
 	}
 }
 

@@ -521,6 +521,15 @@ def test_adjust_offsets_outside_the_ids():
 
 # ------------------------------------------------------------------ together, streams, graphs
 
+def test_adjust_as_many_queries_as_an_int_counts():
+    n = 2**31 - 1
+    s = torch.zeros(n + 64, 1, dtype=F16, device="cuda")
+    nd.adjust_scores(s[:n], bias=torch.ones(1, device="cuda"), out=s[:n])
+    for q in range(0, n, 1 << 28):
+        assert bool((s[q:min(q + (1 << 28), n)] == 1).all()), q
+    assert not bool(s[n:].any())
+
+
 def test_scores_adjusted_and_ranked_are_the_search():
     """the way a session is served: the product, the rows it has been given pushed down, a filter — and, where there is only
     a bias and a filter, the search that does it in one call"""
