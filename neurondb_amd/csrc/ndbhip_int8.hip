@@ -2101,9 +2101,15 @@ ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const f
 		return NDBHIP_OK;
 	if (t->n == 0)
 	{
-		const uint64_t m = (uint64_t) nq * k;
+		const uint64_t all = (uint64_t) nq * k, slab = (uint64_t) 1 << 31;
 
-		hipLaunchKernelGGL(k_i8_none, dim3((unsigned) ((m + 255) / 256)), dim3(256), 0, g.stream, d_ids, d_scores, m);
+		/* (HIP counts a grid's threads in 32 bits) */
+		for (uint64_t e = 0; e < all; e += slab)
+		{
+			const uint64_t m = std::min(slab, all - e);
+
+			hipLaunchKernelGGL(k_i8_none, dim3((unsigned) ((m + 255) / 256)), dim3(256), 0, g.stream, d_ids + e, d_scores + e, m);
+		}
 		HIP_TRY(hipGetLastError());
 		return NDBHIP_OK;
 	}

@@ -397,6 +397,15 @@ def test_search_of_an_empty_table_and_of_no_queries():
     assert t.scores(torch.ones(0, 8, device="cuda")).shape == (0, 5)
 
 
+def test_search_of_an_empty_table_with_more_places_than_a_grid_has_threads():
+    nq, k = 2**22 + 1, 1024
+    ids, sc = nd.Int8Table(1).search(torch.zeros(nq, 1, device="cuda"), k)
+    for q in range(0, nq, 1 << 18):
+        assert bool((ids[q:q + (1 << 18)] == -1).all()) and bool((sc[q:q + (1 << 18)] == -math.inf).all()), q
+    del ids, sc
+    torch.cuda.empty_cache()
+
+
 def test_search_more_queries_than_one_pass_takes():
     n, dim, nq = 300, 32, 9001
     rows, q = rand(1, n, dim), rand(2, nq, dim)
