@@ -104,6 +104,28 @@ def test_quantise(dim, dtype):
     assert bool(scales[2:4].isnan().all()) and not codes[1:4].any()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim", [1, 3, 5, 8, 9, 31, 100, 128, 255, 256, 257, 300, 505, 512, 513, 1000, 1024, 1025, 1100])
+def test_many_rows_there_and_back(dim, dtype):
+    """as many rows as several are quantised a lane at, in a matrix with a border that stays as it is"""
+    n = 6 * 256 * 256 // min(64, 1 << max(0, (dim * (4 if dtype == F32 else 2) - 1) // 16).bit_length()) + 3
+    x = rand(dim, n, dim, dtype=dtype)
+    x[n // 2] = 0
+    x[n - 1, dim // 2] = math.nan
+    c = torch.full((n + 9, dim + 5), 77, dtype=torch.int8, device="cuda")
+    s = torch.full((n + 9,), 77.0, device="cuda")
+    nd.quantize_rows(x.cuda(), c[:n, 2:dim + 2], s[:n])
+    rc, rs = quantise(x)
+    same(c[:n, 2:dim + 2], rc)
+    same(s[:n], rs)
+    out = torch.full((n + 9, dim + 3), 77.0, dtype=dtype, device="cuda")
+    nd.dequantize_rows(c[:n, 2:dim + 2], s[:n], out=out[:n, 1:dim + 1])
+    same(out[:n, 1:dim + 1], (rc.float() * rs[:, None]).to(dtype))
+    assert bool((c[n:] == 77).all()) and bool((c[:, :2] == 77).all()) and bool((c[:, dim + 2:] == 77).all())
+    assert bool((s[n:] == 77).all())
+    assert bool((out[n:] == 77).all()) and bool((out[:, :1] == 77).all()) and bool((out[:, dim + 1:] == 77).all())
+
+
 def test_quantise_halves_tiny_and_huge_values():
     half = torch.arange(-127, 128, dtype=F32)[None].repeat(2, 1)
     half[0, 1:-1] += 0.5                    # top = 127, inv = 1: every product is a half, ties to even
