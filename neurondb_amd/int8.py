@@ -8,18 +8,35 @@ and can be captured into a graph (the workspace of a call comes from torch's all
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
+import os
 import threading
 
 import numpy as np
 
 from . import _lib
-from ._lib import ERR_INVALID, NdbHipError, check, ensure_init, lib
+from ._lib import ERR_INVALID, ERR_NODEVICE, NdbHipError, check, ensure_init, lib
 
 STREAM_LEGACY = 1           # NDBHIP_STREAM_LEGACY: the default stream, whose own handle is 0
 
 
 def _bad(msg):
     return NdbHipError(ERR_INVALID, msg)
+
+
+def _native(device):
+    """csrc/ndb_torch.cpp: the calls whose host time is what they cost, in one crossing; tensors are to be on `device`"""
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_ndb_torch.so")
+    if not os.path.exists(path):
+        raise NdbHipError(ERR_NODEVICE, f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    loader = importlib.machinery.ExtensionFileLoader("_ndb_torch", path)
+    m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ndb_torch", loader))
+    loader.exec_module(m)
+    L = lib()
+    m.setup(NdbHipError, str(device), *(C.cast(f, C.c_void_p).value for f in
+                                        (L.ndbhip_swap_thread_stream, L.ndbhip_last_error, L.ndbhip_scores_adjust_device)))
+    return m
 
 
 class _Torch:
@@ -40,6 +57,7 @@ class _Torch:
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         index = _lib._device
         self.stream = (lambda: raw(index)) if raw else (lambda: torch.cuda.current_stream(index).cuda_stream)
+        self.adjust = _native(self.device).adjust
 
 
 _state = None
@@ -156,15 +174,12 @@ def _mask_arg(mask, nq, n):
     return m, 0 if m.shape[0] == 1 else stride
 
 
-def _bias_arg(bias, nq, n, per_query):
+def _bias_arg(bias, n):
     if bias is None:
-        return None, 0
-    _tensor(bias, "bias", _state.f32, (1, 2) if per_query else 1)
-    b = bias[None] if bias.dim() == 1 else bias
-    if b.shape[0] not in (1, nq) or b.shape[1] != n:
-        raise _bad(f"bias must be [{n}]" + (f" or [1 or {nq}, {n}]" if per_query else ""))
-    b, stride = _rows(b)
-    return b, 0 if b.shape[0] == 1 else stride
+        return None
+    if _tensor(bias, "bias", _state.f32, 1).shape[0] != n:
+        raise _bad(f"bias must be [{n}]")
+    return bias.contiguous()
 
 
 def adjust_scores(scores, seen=None, penalties=None, bias=None, mask=None, out=None):
@@ -176,37 +191,8 @@ def adjust_scores(scores, seen=None, penalties=None, bias=None, mask=None, out=N
     mask       int32 words [ceil(n / 32)] or [nq, ceil(n / 32)], bit i % 32 of word i / 32: 0 = -inf
     out        another tensor of the scores' shape and type, or `scores` itself (in place); None: a new one
     """
-    T = _torch()
-    _tensor(scores, "scores", T.floats, 2)
-    nq, n = scores.shape
-    if out is not None:
-        _tensor(out, "out", (scores.dtype,), 2)
-        if out.shape != scores.shape:
-            raise _bad("out must have the scores' shape")
-        ostride = _out_rows(out, "out")
-    src, stride = _rows(scores)
-    if out is None:
-        out = T.torch.empty((nq, n), dtype=scores.dtype, device=T.device)
-        ostride = n
-    off = ids = None
-    nids = 0
-    if (seen is None) != (penalties is None):
-        raise _bad("seen and penalties go together")
-    if seen is not None:
-        off, ids = seen
-        off = _tensor(off, "offsets", T.i64, 1).contiguous()
-        ids = _tensor(ids, "ids", T.i32, 1).contiguous()
-        penalties = _tensor(penalties, "penalties", T.f32, 2).contiguous()
-        if off.shape[0] != nq + 1 or penalties.shape != (nq, 3):
-            raise _bad("offsets must be [nq + 1] and penalties [nq, 3]")
-        nids = ids.numel()
-        if nids == 0:
-            off = ids = penalties = None
-    bias, bstride = _bias_arg(bias, nq, n, True)
-    mask, mstride = _mask_arg(mask, nq, n)
-    _call(T.lib.ndbhip_scores_adjust_device, _p(src), T.types[src.dtype], nq, n, stride, _p(off), _p(ids), nids, _p(penalties), _p(bias), bstride,
-          _p(mask), mstride, _p(out), ostride)
-    return out
+    T = _state or _torch()
+    return T.adjust(T.stream() or STREAM_LEGACY, scores, seen, penalties, bias, mask, out)
 
 
 class Int8Table:
@@ -308,7 +294,7 @@ class Int8Table:
         float32, float16, bfloat16, or (codes, scales)."""
         T, q, stride, qs = self._queries(queries)
         nq, n = q.shape[0], self._n
-        bias, _ = _bias_arg(bias, 1, n, False)
+        bias = _bias_arg(bias, n)
         if out is None:
             out = T.torch.empty((nq, n), dtype=dtype or T.torch.float32, device=T.device)
         _tensor(out, "out", T.floats, 2)
@@ -328,7 +314,7 @@ class Int8Table:
             return self._search_host(queries, int(k), bias, mask)
         T, q, stride, qs = self._queries(queries)
         nq, n, k = q.shape[0], self._n, int(k)
-        bias, _ = _bias_arg(bias, 1, n, False)
+        bias = _bias_arg(bias, n)
         mask, mstride = _mask_arg(mask, nq, n)
         ws, wsb = self._workspace(T, nq, k)
         ids = T.torch.empty((nq, k), dtype=T.torch.int64, device=T.device)

@@ -1,0 +1,32 @@
+"""The way from Python and C to the 8-bit kernels, on the device: what a call costs and leaves behind."""
+import time
+
+import pytest
+import torch
+
+import neurondb_amd as nd
+
+pytestmark = pytest.mark.gpu
+
+
+def us(calls, reps=300, rounds=9):
+    """the least time a call of each took, back to back, the calls' rounds taking turns"""
+    best = [float("inf")] * len(calls)
+    for _ in range(rounds):
+        for i, c in enumerate(calls):
+            c()
+            torch.cuda.synchronize()
+            t = time.perf_counter()
+            for _ in range(reps):
+                c()
+            torch.cuda.synchronize()
+            best[i] = min(best[i], (time.perf_counter() - t) / reps * 1e6)
+    return best
+
+
+@pytest.mark.parametrize("nq,n", [(1, 1), (1, 10_000), (16, 3000)])
+def test_one_term_on_few_scores_costs_no_more_than_an_addition(nq, n):
+    """a third is left for the noise of a shared host; a call in several crossings took 1.8 to 2 times the addition"""
+    s, b = torch.randn(nq, n, device="cuda"), torch.randn(n, device="cuda")
+    own, plain = us([lambda: nd.adjust_scores(s, bias=b), lambda: s + b[None]])
+    assert own < 1.33 * plain, (own, plain)
