@@ -758,6 +758,7 @@ int			ndbhip_quant_fp16(const float *in, uint16_t *out, int64_t n);
  * (ndbhip_i8_workspace; 256-byte aligned; its contents mean nothing before or after, and it must live until the call's kernels
  * have run — for a captured graph, as long as the graph is replayed).  ndbhip_i8_load* and _destroy wait for nothing but
  * their own work: call them while no other call on the table is in flight and no graph that reads it will be replayed.
+ * The calling thread's current HIP device is the same after a call as before it.
  * Any dimension 1 .. 32767, any number of rows below 2^31 - 256, any strides and alignments of an element's own size. */
 /* ------------------------------------------------------------------ */
 typedef struct ndbhip_i8 ndbhip_i8;		/* device-resident table of 8-bit rows */

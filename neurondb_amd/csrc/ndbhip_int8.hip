@@ -1566,6 +1566,24 @@ k_scores_adjust(const I8Adjust a)
 /* host                                                                */
 /* ================================================================== */
 
+/* The library's device for as long as a call runs, and the caller's own again behind it: calls on torch tensors come from
+ * programs that keep HIP's current device for themselves. */
+struct I8Device
+{
+	int			callers = -1;
+	int enter()
+	{
+		if (g.inited && hipGetDevice(&callers) != hipSuccess)
+			callers = -1;
+		return need_init();
+	}
+	~I8Device()
+	{
+		if (callers >= 0 && callers != g.device)
+			(void) hipSetDevice(callers);
+	}
+};
+
 struct ndbhip_i8
 {
 	int			dim = 0;
@@ -1689,7 +1707,9 @@ ndbhip_i8_quantize_device(const void *d_x, int dtype, int64_t nrows, int dim, in
 		return fail(NDBHIP_ERR_INVALID, "bad sizes");
 	if (nrows > 0 && (!d_x || !d_codes || !d_scales))
 		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	if (nrows == 0)
 		return NDBHIP_OK;
 	return i8_quantize_any<false>(d_x, dtype, nrows, nrows, dim, x_stride, (unsigned char *) d_codes, codes_stride, 0, d_scales);
@@ -1742,7 +1762,9 @@ ndbhip_i8_dequantize_device(const int8_t *d_codes, int64_t codes_stride, const f
 		return fail(NDBHIP_ERR_INVALID, "bad sizes");
 	if (nrows > 0 && (!d_codes || !d_scales || !d_out))
 		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	if (nrows == 0)
 		return NDBHIP_OK;
 	if (dtype == NDBHIP_F32)
@@ -1793,7 +1815,9 @@ ndbhip_i8_destroy(ndbhip_i8 *t)
 {
 	if (!t)
 		return NDBHIP_OK;
-	if (t->d_codes && need_init())
+	I8Device	dev;
+
+	if (t->d_codes && dev.enter())
 		return NDBHIP_ERR_NODEVICE;
 	const int	rc = i8_clear(t);
 
@@ -1836,7 +1860,9 @@ ndbhip_i8_load_device(ndbhip_i8 *t, const void *d_rows, int dtype, int64_t nrows
 		return fail(NDBHIP_ERR_INVALID, "bad sizes");
 	if (nrows > 0 && (!d_rows || (dtype == NDBHIP_I8) != (d_scales != nullptr)))
 		return fail(NDBHIP_ERR_INVALID, "rows are NULL, or scales given for rows that are not NDBHIP_I8 (or none for rows that are)");
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	int			rc = i8_room(t, nrows);
 
 	if (rc || nrows == 0)
@@ -1862,7 +1888,9 @@ ndbhip_i8_load(ndbhip_i8 *t, const float *rows, int64_t nrows)
 		return fail(NDBHIP_ERR_INVALID, "table is NULL");
 	if (nrows < 0 || nrows > I8_MAX_ROWS || (nrows > 0 && !rows))
 		return fail(NDBHIP_ERR_INVALID, "bad arguments");
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	int			rc = i8_room(t, nrows);
 
 	if (rc || nrows == 0)
@@ -1903,7 +1931,9 @@ ndbhip_i8_export_device(const ndbhip_i8 *t, int8_t *d_codes, int64_t codes_strid
 		return fail(NDBHIP_ERR_INVALID, "table is NULL");
 	if (t->n > 0 && (!d_codes || !d_scales || codes_stride < t->dim))
 		return fail(NDBHIP_ERR_INVALID, "bad arguments");
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	if (t->n == 0)
 		return NDBHIP_OK;
 	const int64_t slab = i8_slab_rows(t->dim);
@@ -2140,7 +2170,9 @@ ndbhip_i8_product_device(const ndbhip_i8 *t, const void *d_q, int q_type, const 
 		return fail(NDBHIP_ERR_INVALID, "out is NULL");
 	if (nq > 0 && t->n > 0 && (rc = i8_check_ws(t, nq, 0, d_ws, ws_bytes)))
 		return rc;
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	if (nq == 0 || t->n == 0)
 		return NDBHIP_OK;
 	const int	chunk = i8_chunk(t, nq, 0);
@@ -2191,7 +2223,9 @@ ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const f
 		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
 	if (nq > 0 && t->n > 0 && (rc = i8_check_ws(t, nq, k, d_ws, ws_bytes)))
 		return rc;
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	if (nq == 0)
 		return NDBHIP_OK;
 	if (t->n == 0)
@@ -2269,7 +2303,9 @@ ndbhip_i8_search(const ndbhip_i8 *t, const float *queries, int nq, const float *
 		return fail(NDBHIP_ERR_INVALID, "mask_stride must be 0 (one mask) or at least a word for every 32 rows");
 	if (nq > 0 && (!queries || !ids || !scores))
 		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	if (nq == 0)
 		return NDBHIP_OK;
 	size_t		wsb = 0;
@@ -2352,7 +2388,9 @@ ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, 
 		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
 	if (nq > 1 && d_scores == d_out && stride != out_stride)
 		return fail(NDBHIP_ERR_INVALID, "in place, the two strides must be the same");
-	if (need_init()) return NDBHIP_ERR_NODEVICE;
+	I8Device	dev;
+
+	if (dev.enter()) return NDBHIP_ERR_NODEVICE;
 	if (nq == 0 || n == 0)
 		return NDBHIP_OK;
 	const I8Adjust a = {d_scores, stride, n, d_seen_off, d_seen_ids, n_seen, d_penalties, d_bias, bias_stride, d_mask, mask_stride, d_out,

@@ -11,6 +11,7 @@ import ctypes as C
 import importlib.machinery
 import importlib.util
 import os
+import sys
 import threading
 
 import numpy as np
@@ -202,6 +203,11 @@ class Int8Table:
     order into the L2 one."""
 
     def __init__(self, dim: int, device: int | None = None):
+        if device is None and not _lib._inited:
+            # the device of the tensors it is going to meet, where the program has taken one up; else the process's own
+            cuda = getattr(sys.modules.get("torch"), "cuda", None)
+            if cuda is not None and cuda.is_initialized():
+                device = cuda.current_device()
         ensure_init(device)
         self.dim = int(dim)
         h = C.c_void_p()

@@ -59,3 +59,16 @@ def test_adjust_takes_what_it_can_read(adjust):
     ]
     for i, c in enumerate(good):
         assert code_of(c) == _lib.ERR_NODEVICE, i
+
+
+@pytest.mark.parametrize("taken_up,want", [(True, 1), (False, None)])
+def test_a_table_is_on_the_device_of_the_tensors_it_will_meet(monkeypatch, taken_up, want):
+    """as the first call of a process: torch's current device, as the calls on tensors take, or, without one, the process's own"""
+    asked = []
+    monkeypatch.setattr(_lib, "_inited", False)
+    monkeypatch.setattr(int8, "ensure_init", asked.append)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: taken_up)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    int8.Int8Table(8).close()
+    int8.Int8Table(8, device=0).close()
+    assert asked == [want, 0]
