@@ -11,6 +11,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <cstdarg>
 #include <cstdio>
@@ -95,6 +96,8 @@ tensor(PyObject *o, const char *name, int types, int ndim, int ndim2 = -1)
 		refuse("%s must be a dense tensor", name);
 	if (t.dim() != ndim && t.dim() != ndim2)
 		refuse("%s has %d dimensions", name, (int) t.dim());
+	if (t.requires_grad() && at::GradMode::is_enabled())
+		refuse("%s requires a gradient, which this call has none of: detach() it, or call under no_grad()", name);
 	return t;
 }
 
@@ -216,7 +219,13 @@ adjust(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 		Py_END_ALLOW_THREADS
 		if (rc)
 			raise(rc, g_last_error());
-		return oout != Py_None ? (Py_INCREF(oout), oout) : THPVariable_Wrap(std::move(made));
+		if (oout == Py_None)
+			return THPVariable_Wrap(std::move(made));
+		/* (what autograd has saved of the caller's tensor is another version now) */
+		if (!made.is_inference())
+			made.unsafeGetTensorImpl()->bump_version();
+		Py_INCREF(oout);
+		return oout;
 	}
 	catch (const Refused &)
 	{

@@ -4,6 +4,9 @@ rows of a table.
 
 Everything here takes and returns torch tensors on the device the library runs on, is ordered on torch's current stream
 and can be captured into a graph (the workspace of a call comes from torch's allocator; a graph owns its own).
+
+No call has a gradient.  A tensor that requires one is refused while autograd follows it, so that none is lost unseen
+(detach() it, or call under no_grad()); the rows a table is loaded with are copied, and may be such tensors.
 """
 from __future__ import annotations
 
@@ -52,6 +55,7 @@ class _Torch:
         self.floats = (torch.float32, torch.float16, torch.bfloat16)
         self.f32, self.i8, self.i32, self.i64 = (torch.float32,), (torch.int8,), (torch.int32,), (torch.int64,)
         self.words = (torch.int32, torch.uint32) if hasattr(torch, "uint32") else (torch.int32,)
+        self.increment_version = torch.autograd.graph.increment_version
         self.device = torch.device("cuda", _lib._device)
         self.lib = lib()
         # torch's own short cut to the current stream's handle (0.1 us, against 1.7 us through a Stream object)
@@ -95,8 +99,8 @@ def _call(fn, *args):
         swap(prev, ref)
 
 
-def _tensor(t, name, dtypes, ndim):
-    """checks what every tensor argument has to be"""
+def _tensor(t, name, dtypes, ndim, followed=False):
+    """checks what every tensor argument has to be; followed: it may be one whose gradients autograd is to find"""
     T = _state
     if not isinstance(t, T.torch.Tensor):
         raise _bad(f"{name} must be a torch tensor")
@@ -106,7 +110,16 @@ def _tensor(t, name, dtypes, ndim):
         raise _bad(f"{name} must be one of {[str(d) for d in dtypes]}, not {t.dtype}")
     if t.dim() != ndim and (type(ndim) is int or t.dim() not in ndim):
         raise _bad(f"{name} has {t.dim()} dimensions")
+    if t.requires_grad and not followed and T.torch.is_grad_enabled():
+        raise _bad(f"{name} requires a gradient, which this call has none of: detach() it, or call under no_grad()")
     return t
+
+
+def _written(*out):
+    """the caller's own tensors that a call has written into: what autograd has saved of them is another version now"""
+    for t in out:
+        if not t.is_inference():
+            _state.increment_version(t)
 
 
 def _rows(t):
@@ -131,6 +144,7 @@ def quantize_rows(x, codes=None, scales=None):
     T = _torch()
     x, stride = _rows(_tensor(x, "x", T.floats, 2))
     n, dim = x.shape
+    given = [t for t in (codes, scales) if t is not None]
     if codes is None:
         codes = T.torch.empty((n, dim), dtype=T.torch.int8, device=T.device)
         cstride = dim
@@ -143,6 +157,7 @@ def quantize_rows(x, codes=None, scales=None):
     if codes.shape != x.shape or scales.shape[0] != n or not scales.is_contiguous():
         raise _bad("codes must be [n, dim] and scales [n], contiguous")
     _call(T.lib.ndbhip_i8_quantize_device, _p(x), T.types[x.dtype], n, dim, stride, _p(codes), cstride, _p(scales))
+    _written(*given)
     return codes, scales
 
 
@@ -154,12 +169,14 @@ def dequantize_rows(codes, scales, dtype=None, out=None):
     n, dim = codes.shape
     if scales.shape[0] != n:
         raise _bad("a scale for every row")
+    given = () if out is None else (out,)
     if out is None:
         out = T.torch.empty((n, dim), dtype=dtype or T.torch.float32, device=T.device)
     _tensor(out, "out", T.floats, 2)
     if out.shape != codes.shape or dtype not in (None, out.dtype):
         raise _bad("out must have the codes' shape and the dtype asked for")
     _call(T.lib.ndbhip_i8_dequantize_device, _p(codes), stride, _p(scales), n, dim, _p(out), T.types[out.dtype], _out_rows(out, "out"))
+    _written(*given)
     return out
 
 
@@ -250,13 +267,13 @@ class Int8Table:
                 self._loaded()
             return
         T = _torch()
-        r, stride = _rows(_tensor(rows, "rows", tuple(T.types), 2))
+        r, stride = _rows(_tensor(rows, "rows", tuple(T.types), 2, followed=True))
         if r.shape[1] != self.dim:
             raise _bad(f"rows must be [n, {self.dim}]")
         if (r.dtype == T.torch.int8) != (scales is not None):
             raise _bad("scales go with int8 rows, and only with them")
         if scales is not None:
-            scales = _tensor(scales, "scales", T.f32, 1).contiguous()
+            scales = _tensor(scales, "scales", T.f32, 1, followed=True).contiguous()
             if scales.shape[0] != r.shape[0]:
                 raise _bad("a scale for every row")
         try:
@@ -301,6 +318,7 @@ class Int8Table:
         T, q, stride, qs = self._queries(queries)
         nq, n = q.shape[0], self._n
         bias = _bias_arg(bias, n)
+        given = () if out is None else (out,)
         if out is None:
             out = T.torch.empty((nq, n), dtype=dtype or T.torch.float32, device=T.device)
         _tensor(out, "out", T.floats, 2)
@@ -310,6 +328,7 @@ class Int8Table:
         ws, wsb = self._workspace(T, nq, 0)
         _call(T.lib.ndbhip_i8_product_device, self._h, _p(q), T.types[q.dtype], _p(qs), nq, stride, _p(bias), _p(out), T.types[out.dtype],
               ostride, _p(ws), wsb)
+        _written(*given)
         return out
 
     def search(self, queries, k, bias=None, mask=None):

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import neurondb_amd as nd
+from neurondb_amd._lib import NdbHipError
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +31,24 @@ def test_one_term_on_few_scores_costs_no_more_than_an_addition(nq, n):
     s, b = torch.randn(nq, n, device="cuda"), torch.randn(n, device="cuda")
     own, plain = us([lambda: nd.adjust_scores(s, bias=b), lambda: s + b[None]])
     assert own < 1.33 * plain, (own, plain)
+
+
+def test_a_saved_tensor_is_not_changed_unseen():
+    """scores that some backward has kept, adjusted in place: autograd says so instead of using the new ones"""
+    s = torch.randn(3, 50, device="cuda")
+    w = torch.ones(3, 50, device="cuda", requires_grad=True)
+    loss = (w * s).sum()
+    nd.adjust_scores(s, bias=torch.ones(50, device="cuda"), out=s)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with pytest.raises(NdbHipError, match="gradient"):
+        nd.adjust_scores(w)
+    with torch.no_grad():
+        assert torch.equal(nd.adjust_scores(w, bias=torch.ones(50, device="cuda")), w + 1)
+    t = nd.Int8Table(50)
+    t.load(w)                               # a copy
+    assert not t.scores(w.detach()).requires_grad
+    with torch.inference_mode():
+        v = torch.ones(3, 3, device="cuda")
+    nd.adjust_scores(v, out=v)
+    t.scores(w.detach(), out=v)

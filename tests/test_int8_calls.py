@@ -72,3 +72,62 @@ def test_a_table_is_on_the_device_of_the_tensors_it_will_meet(monkeypatch, taken
     int8.Int8Table(8).close()
     int8.Int8Table(8, device=0).close()
     assert asked == [want, 0]
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """the module as after its first call, told that the library is on the CPU: a good call ends where the device is asked for"""
+    monkeypatch.setattr(int8, "ensure_init", lambda device=None: None)
+    monkeypatch.setattr(_lib, "_inited", True)
+    monkeypatch.setattr(_lib, "_device", 0)
+    T = int8._Torch()
+    T.device, T.stream, T.adjust = torch.device("cpu"), lambda: 1, int8._native("cpu").adjust
+    monkeypatch.setattr(int8, "_state", T)
+
+
+@no_gpu
+def test_tensors_whose_gradients_would_be_lost_are_refused(on_cpu):
+    """the results carry no graph: an argument that autograd follows is refused while it does"""
+    x, b, s = torch.ones(4, 16), torch.ones(70), torch.ones(4, 70)
+    c, sc, pen = torch.ones(4, 16, dtype=torch.int8), torch.ones(4), torch.ones(4, 3)
+    off, ids = torch.zeros(5, dtype=torch.int64), torch.zeros(2, dtype=torch.int32)
+    g = lambda t: t.clone().requires_grad_()        # noqa: E731
+    t = int8.Int8Table(16)
+    t._n = 70
+    calls = [
+        lambda f: int8.quantize_rows(f(x)), lambda f: int8.quantize_rows(f(x) * 2), lambda f: int8.quantize_rows(x, scales=f(sc)),
+        lambda f: int8.dequantize_rows(c, f(sc)), lambda f: int8.dequantize_rows(c, sc, out=f(x)),
+        lambda f: int8.adjust_scores(f(s)), lambda f: int8.adjust_scores(s, out=f(s)), lambda f: int8.adjust_scores(s, bias=f(b)),
+        lambda f: int8.adjust_scores(s, (off, ids), f(pen)),
+        lambda f: t.scores(f(x)), lambda f: t.scores(x, bias=f(b)), lambda f: t.scores((c, f(sc))), lambda f: t.scores(x, out=f(s)),
+        lambda f: t.search(f(x), 3), lambda f: t.search(x, 3, bias=f(b)), lambda f: t.search((c, f(sc)), 3),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(NdbHipError, match="gradient") as e:
+            call(g)
+        assert e.value.code == _lib.ERR_INVALID, i
+        assert code_of(lambda: call(lambda v: v)) == _lib.ERR_NODEVICE, i
+        with torch.no_grad():
+            assert code_of(lambda: call(g)) == _lib.ERR_NODEVICE, i
+        assert code_of(lambda: call(lambda v: g(v).detach())) == _lib.ERR_NODEVICE, i
+    # a table is a copy: its rows may come from a model that is being trained
+    assert code_of(lambda: t.load(g(x))) == _lib.ERR_NODEVICE
+    t.close()
+
+
+@no_gpu
+def test_what_is_written_into_is_a_new_version(on_cpu, monkeypatch):
+    """a tensor that a call writes into, saved for some backward, is seen to have changed there"""
+    monkeypatch.setattr(int8, "_call", lambda *a: None)
+    x, s, sc = torch.ones(4, 16), torch.ones(4, 70), torch.ones(4)
+    c = torch.ones(4, 16, dtype=torch.int8)
+    t = int8.Int8Table(16)
+    monkeypatch.setattr(t, "_n", 70)
+    for call, outs in ((lambda: int8.quantize_rows(x, c, sc), (c, sc)), (lambda: int8.dequantize_rows(c, sc, out=x), (x,)), (lambda: t.scores(x, out=s), (s,))):
+        before = [o._version for o in outs]
+        call()
+        assert [o._version for o in outs] == [v + 1 for v in before]
+    with torch.inference_mode():
+        still = torch.ones(4, 70)
+    t.scores(x, out=still)                  # (these have no versions)
+    t.close()
