@@ -678,24 +678,29 @@ i8_wait_vm()
 /* lane i copies 16 (4) bytes at base + voff to LDS at la + 16 (4) i.  Inline asm: the compiler would put a wait for ALL
  * such copies in front of every LDS read of a ring it cannot tell apart, and M0, which only these copies use here, is
  * written right before each (the wait states cover M0 and a base that a vector instruction has just put into its scalar
- * registers).  Not a memory clobber: the barriers around the ring are, and copies may move between reads. */
+ * registers).  M0 is named as written: the compiler keeps nothing in it from one instruction to another and so warns, but it
+ * may share one setting of it between instructions, and must not across these.  Not a memory clobber: the barriers around the
+ * ring are, and copies may move between reads. */
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void
 i8_dma16(const void *base, uint32_t voff, uint32_t la)
 {
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(la), "v"(voff), "s"(base));
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(la), "v"(voff), "s"(base) : "m0");
 }
 __device__ __forceinline__ void
 i8_dma4(const void *base, uint32_t voff, uint32_t la)
 {
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" :: "s"(la), "v"(voff), "s"(base));
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" :: "s"(la), "v"(voff), "s"(base) : "m0");
 }
 
 /* the same from 64 unrelated addresses */
 __device__ __forceinline__ void
 i8_dma4_at(const void *p, uint32_t la)
 {
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off" :: "s"(la), "v"(p));
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off" :: "s"(la), "v"(p) : "m0");
 }
+#pragma clang diagnostic pop
 
 template <class T>
 __device__ __forceinline__ T *

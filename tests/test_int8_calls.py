@@ -1,4 +1,7 @@
 """The way from Python and C to the 8-bit kernels, without a device: what the calls on torch tensors refuse."""
+import os
+import re
+
 import pytest
 import torch
 
@@ -131,3 +134,12 @@ def test_what_is_written_into_is_a_new_version(on_cpu, monkeypatch):
         still = torch.ones(4, 70)
     t.scores(x, out=still)                  # (these have no versions)
     t.close()
+
+
+def test_assembly_that_writes_m0_says_so():
+    """M0 is the compiler's too (LDS, relative moves, barriers' messages): inline assembly that writes it has to name it"""
+    src = open(os.path.join(os.path.dirname(int8.__file__), "csrc", "ndbhip_int8.hip")).read()
+    asm = [a for a in re.findall(r"asm volatile\((.*?)\);", src, re.S) if "m0" in a]
+    assert len(asm) == 3
+    for a in asm:
+        assert re.search(r':\s*"m0"\s*$', a), a
