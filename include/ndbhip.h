@@ -784,7 +784,9 @@ int			ndbhip_i8_load_device(ndbhip_i8 *t, const void *d_rows, int dtype, int64_t
 int			ndbhip_i8_export_device(const ndbhip_i8 *t, int8_t *d_codes, int64_t codes_stride, float *d_scales);
 int64_t		ndbhip_i8_nrows(const ndbhip_i8 *t);
 int			ndbhip_i8_dim(const ndbhip_i8 *t);
-/* bytes of workspace for a batch of nq queries: k = 0 for ndbhip_i8_product_device, the search's k for a search */
+/* Bytes of workspace for a batch of nq queries: k = 0 for ndbhip_i8_product_device, the search's k for a search.  Batches go in
+ * passes of up to 4096 queries, a search's in passes that leave it near a gigabyte: 256 queries of more than 27 million rows
+ * take more (40 bytes a row), up to 16 GiB, and then passes are shorter. */
 int			ndbhip_i8_workspace(const ndbhip_i8 *t, int nq, int k, size_t *bytes);
 
 /* every score: d_out[q * out_stride + i], fp32 or rounded once more to 16 bits */

@@ -2013,14 +2013,18 @@ i8_ws(const ndbhip_i8 *t, int nq, int k)
 	return w;
 }
 
-/* queries a search takes at a time: as many as leave its workspace near a gigabyte, in whole tiles */
+/*
+ * Queries a call takes at a time: as many as leave its workspace near a gigabyte, and the wide tile's 256 as long as that is
+ * no more than 16, in whole tiles; a search leaves 5 bytes a query for 32 rows, which hold 68 each at the least.  (256 queries of
+ * 100M x 64, 3.7 GB: 7.8 ms; in passes of 96, 10.9.)  Not below 32, the queries the stream multiplies with one reading of the table.
+ */
 static int
 i8_chunk(const ndbhip_i8 *t, int nq, int k)
 {
-	const size_t per = (size_t) t->kp + (size_t) (t->n + 255) / 32 * 5 + (k > I8_FUSED_K ? (size_t) k * 132 : 0) + 12;
-	const int64_t m = std::max<int64_t>(256, (int64_t) (((size_t) 1 << 30) / per) / 256 * 256);
+	const size_t per = (size_t) t->kp + 12 + (k > 0 ? (size_t) (t->n + 255) / 32 * 5 : 0) + (k > I8_FUSED_K ? (size_t) k * 132 : 0);
+	const size_t m = std::max({((size_t) 1 << 30) / per, std::min<size_t>(((size_t) 16 << 30) / per, 256), (size_t) 32});
 
-	return (int) std::min<int64_t>(nq, std::min<int64_t>(m, 4096));
+	return (int) std::min<size_t>((size_t) nq, std::min<size_t>(m >= 256 ? m / 256 * 256 : m / 32 * 32, 4096));
 }
 
 extern "C" int

@@ -52,3 +52,25 @@ def test_a_saved_tensor_is_not_changed_unseen():
         v = torch.ones(3, 3, device="cuda")
     nd.adjust_scores(v, out=v)
     t.scores(w.detach(), out=v)
+
+
+def test_a_batch_in_passes_that_fill_no_tile():
+    """a table so long that a search's passes are shorter than a tile is wide: as in pieces, and every row finds itself"""
+    n, dim, nq = 460_000_000, 16, 300
+    g = torch.Generator("cuda").manual_seed(1)
+    codes = torch.randint(-127, 128, (n, dim), device="cuda", generator=g, dtype=torch.int8)
+    scales = torch.cat([1 / c.float().norm(dim=1) for c in codes.split(1 << 25)])
+    t = nd.Int8Table(dim)
+    t.load(codes, scales)
+    want = torch.arange(nq, device="cuda") * 1_533_331
+    q = (codes[want], scales[want])
+    assert t._workspace(nd.int8._state, 256, 3)[1] == t._workspace(nd.int8._state, 224, 3)[1] < 16 << 30
+    torch.cuda.empty_cache()
+    ids, sc = t.search(q, 3)
+    for at in range(0, nq, 50):
+        i, s = t.search((q[0][at:at + 50], q[1][at:at + 50]), 3)
+        assert torch.equal(ids[at:at + 50], i) and torch.equal(sc[at:at + 50], s)
+    found = (codes[ids[:, 0]] == q[0]).all(1) | (sc[:, 0] > 1 - 1e-5)      # (another row may lie in the same direction)
+    assert bool(found.all())
+    del codes, scales, t
+    torch.cuda.empty_cache()

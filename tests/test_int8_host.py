@@ -85,3 +85,44 @@ def test_calls_leave_the_current_device_as_it_was(stub):
             stub.stub_set_room(1 << 60)
             assert L.ndbhip_i8_destroy(t) == 0 and device() == 1
     """)
+
+
+def test_workspace_of_long_tables_stays_in_bounds(stub):
+    """a search's passes are cut so that the workspace is about a gigabyte; a tile's 256 queries may take 16"""
+    run(stub, """
+        G = 1 << 30
+        for n, dim in ((1_000, 64), (1_000_000, 768), (27_000_000, 64), (100_000_000, 64), (100_000_000, 768), (500_000_000, 64), (0x7FFFFF00, 64), (0x7FFFFF00, 90)):
+            t = table(dim, n)
+            bound = max(1.02 * G, min(16 * G, 41 * n)) + (64 << 20)
+            for k in (1, 10, 128, 129, 1024):
+                last = 0
+                for nq in (1, 31, 33, 255, 256, 257, 1024, 5000, 2**31 - 1):
+                    w = workspace(t, nq, k)
+                    assert w >= last and w <= bound and w < stub.stub_in_use() * 5 // 8 + G, (n, dim, k, nq, w)
+                    last = w
+            assert workspace(t, 2**31 - 1, 0) <= 4096 * (dim + 64 + 4) + 4096
+            _lib.check(L.ndbhip_i8_destroy(t))
+        assert stub.stub_in_use() < G
+    """)
+
+
+def test_passes(stub):
+    """launches of a call: the queries, then the product, then what picks the best; the table is read no more often than needed"""
+    run(stub, """
+        def product(t, nq, dim, n):
+            before = stub.stub_launches()
+            _lib.check(L.ndbhip_i8_product_device(t, P, 3, P, nq, dim, None, P, 0, n, P, workspace(t, nq, 0)))
+            return stub.stub_launches() - before
+        def search(t, nq, dim, k):
+            before = stub.stub_launches()
+            _lib.check(L.ndbhip_i8_search_device(t, P, 3, P, nq, dim, None, None, 0, k, P, P, P, workspace(t, nq, k)))
+            return stub.stub_launches() - before
+        t = table(768, 10_000_000)
+        assert product(t, 1024, 768, 10_000_000) == 2 and product(t, 4096, 768, 10_000_000) == 2 and product(t, 4097, 768, 10_000_000) == 4
+        t = table(32, 300)
+        assert search(t, 4096, 32, 5) == 3 and search(t, 9001, 32, 5) == 9
+        t = table(64, 100_000_000)              # 256 queries: 3.7 GB
+        assert search(t, 256, 64, 10) == 3 and search(t, 257, 64, 10) == 6
+        t = table(64, 500_000_000)              # 16 GiB: 192 queries a pass
+        assert search(t, 192, 64, 10) == 3 and search(t, 193, 64, 10) == 6
+    """)
