@@ -750,7 +750,7 @@ template <int NWQ> struct I8Tile
 };
 
 template <int NWQ, class KIND>
-__global__ __launch_bounds__(128 * NWQ, NWQ / 2) void
+__global__ __launch_bounds__(128 * NWQ, 2) void
 k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrt, uint32_t nqt, I8Out o)
 {
 	typedef I8Tile<NWQ> TILE;
@@ -2082,8 +2082,9 @@ i8_tile_launch(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &o)
 {
 	typedef I8Tile<NWQ> TILE;
 	const uint32_t nrt = (o.n + 255) / 256, nqt = (o.nq + 32 * TILE::QB - 1) / (32 * TILE::QB);
-	/* as many blocks as the compute units hold (the narrow tile's LDS fits twice without biases and masks), in whole rounds of
-	 * the XCDs, and no more than have a tile */
+	/* as many blocks as the compute units hold, in whole rounds of the XCDs, and no more than have a tile: the narrow tile's LDS fits
+	 * twice without biases and masks, and so, at two waves a SIMD, do its registers (with one wave a SIMD asked for, it took 316 of 512
+	 * and half of the blocks waited for the others to end: 96 x 1M x 64 76 -> 56 us, 384 x 64000 x 768 36 -> 30) */
 	const uint32_t per_cu = NWQ == 2 && !KIND::BIAS && !KIND::MASK ? 2 : 1;
 	const uint32_t blocks = std::min(((uint32_t) g.num_cus & ~7u) * per_cu, (nrt + 7) / 8 * 8 * nqt);
 
@@ -2110,10 +2111,12 @@ i8_stream_launch(const ndbhip_i8 *t, const unsigned char *queries, const I8Out &
 
 /*
  * Up to 64 queries the table's bytes are what counts, and the stream reads them as fast as memory gives them.  Above, a tile pays
- * where there are enough of them to cover its start (scores of fp16; stream / 128-query tile / 256-query tile in us): 96 x
- * 16000 x 768 10.6 / 11.0 / 14.2, 256 x 16000 x 768 14.9 / 12.4 / 15.0, 96 x 64000 x 64 7.5 / 8.6 / 9.7, 256 x 64000 x 64 11.9 / 11.3
- * / 11.2.  The wide tile does a fifth more per query of its width (512 x 256000 x 768: 257 / 163 / 133) but wants a tile for
- * every compute unit (512 x 16000 x 768: 20.2 / 14.5 / 17.1).  What goes past the caches is always many tiles.
+ * where there are enough of them to cover its start (scores of fp16, the queries' way to the block layout with them; stream / 128-query
+ * tile / 256-query tile in us): 96 x 16000 x 768 12.9 / 13.3 / 16.5, 256 x 16000 x 768 17.6 / 14.4 / 17.8, 96 x 64000 x 64 9.3 / 10.3 /
+ * 11.7, 256 x 64000 x 64 14.3 / 13.6 / 13.4.  The wide tile reads the table half as often (256 x 256000 x 768: 136 / 94 / 82) but wants a
+ * tile for every compute unit (512 x 16000 x 768: 23.4 / 16.1 / 18.7) and queries to fill it (384 x 64000 x 768: 57 / 30 / 34).  Over 65 to
+ * 512 queries x 4000 to 1M rows x 64 to 1536 dimensions the rule is within 8 % of the best of the three, but for 128 x 1M x 64,
+ * whose scores are most of the work (67.6 / 82.7 / 100.8).  What goes past the caches is always many tiles.
  */
 template <class KIND>
 static int
