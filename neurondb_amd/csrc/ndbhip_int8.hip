@@ -2381,6 +2381,26 @@ scores_adjust_launch(I8Adjust a)
 	}
 }
 
+/* whether an element of nq rows of `row` bytes, `astride` bytes apart, lies among those at b; astride, bstride >= row > 0 */
+static bool
+i8_overlap(const void *a, int64_t astride, const void *b, int64_t bstride, int nq, int64_t row)
+{
+	const int64_t d = (int64_t) ((uintptr_t) b - (uintptr_t) a);
+
+	if (d >= (nq - 1) * astride + row || -d >= (nq - 1) * bstride + row)
+		return false;
+	/* row i of b against the rows of a that start next before it and behind it; equal strides: one row stands for all */
+	for (int64_t i = 0; i < (astride == bstride ? 1 : nq); i++)
+	{
+		const int64_t at = d + i * bstride, j = at >= 0 ? at / astride : -((-at + astride - 1) / astride);
+
+		for (int64_t r = j; r <= j + 1; r++)
+			if ((astride == bstride ? r > -nq && r < nq : r >= 0 && r < nq) && at < r * astride + row && r * astride < at + row)
+				return true;
+	}
+	return false;
+}
+
 extern "C" int
 ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, int64_t stride, const int64_t *d_seen_off,
 							const int32_t *d_seen_ids, int64_t n_seen, const float *d_penalties, const float *d_bias, int64_t bias_stride,
@@ -2400,6 +2420,10 @@ ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, 
 		return fail(NDBHIP_ERR_INVALID, "NULL pointer");
 	if (nq > 1 && d_scores == d_out && stride != out_stride)
 		return fail(NDBHIP_ERR_INVALID, "in place, the two strides must be the same");
+	if (nq > 0 && n > 0 && d_scores != d_out &&
+		i8_overlap(d_scores, (nq > 1 ? stride : n) * i8_type_size(dtype), d_out, (nq > 1 ? out_stride : n) * i8_type_size(dtype), nq,
+				   n * i8_type_size(dtype)))
+		return fail(NDBHIP_ERR_INVALID, "out and scores overlap");
 	I8Device	dev;
 
 	if (dev.enter()) return NDBHIP_ERR_NODEVICE;

@@ -207,7 +207,8 @@ def adjust_scores(scores, seen=None, penalties=None, bias=None, mask=None, out=N
     penalties  float32 [nq, 3] = repeat, presence, frequency of each query (with `seen`)
     bias       float32 [n] or [nq, n]
     mask       int32 words [ceil(n / 32)] or [nq, ceil(n / 32)], bit i % 32 of word i / 32: 0 = -inf
-    out        another tensor of the scores' shape and type, or `scores` itself (in place); None: a new one
+    out        another tensor of the scores' shape and type that shares no element with them, or `scores` itself (in place);
+               None: a new one
     """
     T = _state or _torch()
     return T.adjust(T.stream() or STREAM_LEGACY, scores, seen, penalties, bias, mask, out)

@@ -143,3 +143,22 @@ def test_assembly_that_writes_m0_says_so():
     assert len(asm) == 3
     for a in asm:
         assert re.search(r':\s*"m0"\s*$', a), a
+
+
+@no_gpu
+def test_adjust_refuses_a_result_that_overlaps_the_scores():
+    """blocks of threads read and write at the same time: a shared element would be read before or after it is written.  Rows
+    of one buffer that lie between each other are apart."""
+    def call(nq, n, stride, at, ostride, dtype=0):
+        s = 4 if dtype == 0 else 2
+        return L.ndbhip_scores_adjust_device(1 << 20, dtype, nq, n, stride, None, None, 0, None, None, 0, None, 0, (1 << 20) + at * s, ostride)
+    for dtype in (0, 1, 2):
+        for args in ((4, 70, 70, 1, 70), (4, 70, 70, -1, 70), (4, 70, 70, 70, 70), (4, 70, 70, -210, 70), (4, 70, 140, 69, 140), (4, 70, 140, -69, 140),
+                     (4, 70, 140, 70, 70), (4, 70, 70, 0, 71), (2, 70, 1000, 999, 70), (3, 70, 1000, 70, 965), (3, 70, 1000, 70, 900), (1, 70, 70, 69, 70), (1, 70, 70, -69, 70)):
+            assert call(*args, dtype) == _lib.ERR_INVALID, args
+            assert "overlap" in _lib.last_error() or "in place" in _lib.last_error()
+        for args in ((4, 70, 70, 0, 70), (1, 70, 70, 0, 99), (4, 70, 70, 280, 70), (4, 70, 70, -280, 70), (4, 70, 140, 70, 140), (4, 70, 140, -70, 140),
+                     (4, 70, 210, 140, 210), (2, 70, 1000, 70, 70), (3, 70, 1000, 70, 1100), (1, 70, 70, 70, 70), (1, 70, 70, -70, 70)):
+            assert call(*args, dtype) == _lib.ERR_NODEVICE, args
+    # (2^31 rows: neither a long search nor an overflow)
+    assert call(2**31 - 1, 1, 2, 1, 2) == _lib.ERR_NODEVICE and call(2**31 - 1, 2, 2, 1, 2) == _lib.ERR_INVALID
