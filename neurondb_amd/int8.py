@@ -135,6 +135,14 @@ def _out_rows(t, name):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _int(v, name):
+    """a number for a C int, which would silently take the low 32 bits of a larger one"""
+    v = int(v)
+    if not -1 << 31 <= v < 1 << 31:
+        raise _bad(f"{name} is {v}")
+    return v
+
+
 def _p(t):
     return None if t is None else t.data_ptr()
 
@@ -227,7 +235,7 @@ class Int8Table:
             if cuda is not None and cuda.is_initialized():
                 device = cuda.current_device()
         ensure_init(device)
-        self.dim = int(dim)
+        self.dim = _int(dim, "dim")
         h = C.c_void_p()
         check(lib().ndbhip_i8_create(self.dim, C.byref(h)))
         self._h = h
@@ -301,6 +309,7 @@ class Int8Table:
             raise _bad(f"queries must be [nq, {self.dim}]")
         if (q.dtype == T.torch.int8) != (scales is not None) or scales is not None and scales.shape[0] != q.shape[0]:
             raise _bad("int8 queries come as (codes [nq, dim], scales [nq]), others alone")
+        _int(q.shape[0], "the number of queries")
         return T, q, stride, scales
 
     def _workspace(self, T, nq, k):
@@ -337,9 +346,9 @@ class Int8Table:
         no row fills hold -1 and -inf.  ndbhip_i8_search_device.  bias: float32 [nrows]; mask: as in adjust_scores.  numpy float32
         queries (and numpy bias, mask uint32 / int32) take the host form and return numpy arrays."""
         if isinstance(queries, np.ndarray):
-            return self._search_host(queries, int(k), bias, mask)
+            return self._search_host(queries, _int(k, "k"), bias, mask)
         T, q, stride, qs = self._queries(queries)
-        nq, n, k = q.shape[0], self._n, int(k)
+        nq, n, k = q.shape[0], self._n, _int(k, "k")
         bias = _bias_arg(bias, n)
         mask, mstride = _mask_arg(mask, nq, n)
         ws, wsb = self._workspace(T, nq, k)
@@ -354,6 +363,7 @@ class Int8Table:
         n = self._n
         if q.ndim != 2 or q.shape[1] != self.dim:
             raise _bad(f"queries must be [nq, {self.dim}]")
+        _int(q.shape[0], "the number of queries")
         p = lambda a: None if a is None else a.ctypes.data_as(C.c_void_p)     # noqa: E731
         if bias is not None:
             bias = np.ascontiguousarray(bias, dtype=np.float32)

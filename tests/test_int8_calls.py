@@ -162,3 +162,19 @@ def test_adjust_refuses_a_result_that_overlaps_the_scores():
             assert call(*args, dtype) == _lib.ERR_NODEVICE, args
     # (2^31 rows: neither a long search nor an overflow)
     assert call(2**31 - 1, 1, 2, 1, 2) == _lib.ERR_NODEVICE and call(2**31 - 1, 2, 2, 1, 2) == _lib.ERR_INVALID
+
+
+@no_gpu
+def test_counts_that_no_int_holds_are_refused(on_cpu):
+    """a C int takes the low 32 bits of a number: 2^32 + 5 would be 5"""
+    assert code_of(lambda: int8.Int8Table(2**32 + 16)) == _lib.ERR_INVALID
+    t = int8.Int8Table(1)
+    t._n = 70
+    few, many = torch.ones(4, 1), torch.empty(2**32 + 4, 1, dtype=torch.float16)
+    for k in (2**32 + 5, -2**32 + 5):
+        assert code_of(lambda: t.search(few, k)) == _lib.ERR_INVALID
+        assert code_of(lambda: t.search(few.numpy(), k)) == _lib.ERR_INVALID
+    assert code_of(lambda: t.search(few, 5)) == _lib.ERR_NODEVICE
+    assert code_of(lambda: t.search(many, 5)) == _lib.ERR_INVALID
+    assert code_of(lambda: t.scores(many)) == _lib.ERR_INVALID
+    t.close()
