@@ -246,6 +246,7 @@ class Int8Table:
         if getattr(self, "_h", None):
             check(lib().ndbhip_i8_destroy(self._h))
             self._h = None
+            self._loaded()
 
     def __del__(self):
         try:
@@ -258,7 +259,7 @@ class Int8Table:
         return self._n
 
     def _loaded(self):
-        self._n = int(lib().ndbhip_i8_nrows(self._h))
+        self._n = max(int(lib().ndbhip_i8_nrows(self._h)), 0)        # (-1: closed)
         self._ws.clear()
 
     def load(self, rows, scales=None):

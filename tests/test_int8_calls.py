@@ -178,3 +178,18 @@ def test_counts_that_no_int_holds_are_refused(on_cpu):
     assert code_of(lambda: t.search(many, 5)) == _lib.ERR_INVALID
     assert code_of(lambda: t.scores(many)) == _lib.ERR_INVALID
     t.close()
+
+
+@no_gpu
+def test_a_closed_table_refuses_and_stays_empty(on_cpu):
+    import numpy as np
+    t = int8.Int8Table(4)
+    t._n = 70
+    t.close()
+    t.close()
+    assert t.nrows == 0
+    x = torch.ones(3, 4)
+    for call in (lambda: t.load(x), lambda: t.load(np.ones((3, 4), np.float32)), lambda: t.search(x, 3), lambda: t.search(x.numpy(), 3),
+                 lambda: t.scores(x), lambda: t.export()):
+        assert code_of(call) in (_lib.ERR_INVALID, _lib.ERR_NODEVICE)       # (the calls on tensors ask for the device first)
+        assert t.nrows == 0
