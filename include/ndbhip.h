@@ -798,7 +798,8 @@ int			ndbhip_i8_product_device(const ndbhip_i8 *t, const void *d_q, int q_type, 
 int			ndbhip_i8_search_device(const ndbhip_i8 *t, const void *d_q, int q_type, const float *d_q_scales, int nq, int64_t q_stride,
 									const float *d_bias, const uint32_t *d_mask, int64_t mask_stride, int k, int64_t *d_ids, float *d_scores,
 									void *d_ws, size_t ws_bytes);
-/* the same for host queries [nq][dim] and host bias, mask and results */
+/* The same for host queries [nq][dim] and host bias, mask and results.  The table keeps what such searches work in on the device, up
+ * to a gigabyte for each that ran at the same time, until it is loaded again or destroyed. */
 int			ndbhip_i8_search(const ndbhip_i8 *t, const float *queries, int nq, const float *bias, const uint32_t *mask, int64_t mask_stride,
 							 int k, int64_t *ids, float *scores);
 

@@ -5,10 +5,12 @@
  */
 #include <hip/hip_runtime_api.h>
 #include <atomic>
+#include <chrono>
 #include <cstdlib>
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <thread>
 
 static thread_local int t_device;
 static thread_local hipError_t t_last;
@@ -17,7 +19,7 @@ static std::map<char *, size_t> live;
 static size_t in_use, most, room = ~(size_t) 0;
 static char *next_address = (char *) 0x100000000000;
 static std::atomic<long> mallocs, frees, launches;
-static std::atomic<int> launch_device{-1};
+static std::atomic<int> launch_device{-1}, sync_ms;
 
 static hipError_t
 done(hipError_t e)
@@ -36,6 +38,7 @@ extern "C"
 	size_t		stub_in_use(void) { return in_use; }
 	size_t		stub_most(void) { size_t v = most; most = in_use; return v; }
 	void		stub_set_room(size_t bytes) { room = bytes; }
+	void		stub_set_sync_ms(int ms) { sync_ms = ms; }		/* what waiting for a stream takes */
 
 	hipError_t	hipGetDeviceCount(int *n) { *n = 2; return hipSuccess; }
 	hipError_t	hipSetDevice(int d) { t_device = d; return hipSuccess; }
@@ -49,7 +52,12 @@ extern "C"
 	}
 	hipError_t	hipStreamCreateWithFlags(hipStream_t *s, unsigned) { *s = (hipStream_t) malloc(16); return hipSuccess; }
 	hipError_t	hipStreamDestroy(hipStream_t s) { free(s); return hipSuccess; }
-	hipError_t	hipStreamSynchronize(hipStream_t) { return hipSuccess; }
+	hipError_t	hipStreamSynchronize(hipStream_t)
+	{
+		if (sync_ms)
+			std::this_thread::sleep_for(std::chrono::milliseconds(sync_ms));
+		return hipSuccess;
+	}
 	hipError_t	hipFuncSetAttribute(const void *, hipFuncAttribute, int) { return hipSuccess; }
 	hipError_t	hipGetLastError(void) { hipError_t e = t_last; t_last = hipSuccess; return e; }
 	hipError_t	hipHostMalloc(void **p, size_t n, unsigned) { *p = malloc(n); return hipSuccess; }

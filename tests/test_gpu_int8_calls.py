@@ -1,6 +1,8 @@
 """The way from Python and C to the 8-bit kernels, on the device: what a call costs and leaves behind."""
+import threading
 import time
 
+import numpy as np
 import pytest
 import torch
 
@@ -74,3 +76,34 @@ def test_a_batch_in_passes_that_fill_no_tile():
     assert bool(found.all())
     del codes, scales, t
     torch.cuda.empty_cache()
+
+
+def test_two_threads_search_host_arrays_at_the_same_time():
+    """each with a workspace of its own, kept from search to search and made larger where one is"""
+    n, dim = 20_000, 96
+    t = nd.Int8Table(dim)
+    rng = np.random.default_rng(0)
+    t.load(rng.standard_normal((n, dim)).astype(np.float32))
+    q = [rng.standard_normal((m, dim)).astype(np.float32) for m in (1, 7, 40, 300)]
+    mask = rng.integers(0, 2 ** 32, ((n + 31) // 32,), dtype=np.uint32)
+    bias = rng.standard_normal(n).astype(np.float32)
+    dev = [t.search(torch.from_numpy(x).cuda(), 20, bias=torch.from_numpy(bias).cuda(), mask=torch.from_numpy(mask.view(np.int32)).cuda()) for x in q]
+    want = [(i.cpu().numpy(), s.cpu().numpy()) for i, s in dev]
+    bad = []
+
+    def work(order):
+        try:
+            for _ in range(15):
+                for i in order:
+                    ids, sc = t.search(q[i], 20, bias=bias, mask=mask)
+                    if not (np.array_equal(ids, want[i][0]) and np.array_equal(sc, want[i][1])):
+                        bad.append(i)
+        except Exception as e:          # noqa: BLE001 (reported below)
+            bad.append(e)
+
+    th = [threading.Thread(target=work, args=(o,)) for o in ((0, 1, 2, 3), (3, 1, 0, 2), (2, 0, 3, 1))]
+    [x.start() for x in th]
+    [x.join() for x in th]
+    assert not bad
+    t.load(rng.standard_normal((50, dim)).astype(np.float32))
+    assert t.search(q[0], 3)[0].max() < 50

@@ -126,3 +126,52 @@ def test_passes(stub):
         t = table(64, 500_000_000)              # 16 GiB: 192 queries a pass
         assert search(t, 192, 64, 10) == 3 and search(t, 193, 64, 10) == 6
     """)
+
+
+def test_searches_of_host_arrays_keep_their_workspace(stub):
+    """hipMalloc and hipFree, which waits for everything on the device, are for the first search and for larger ones only; searches
+    at the same time have a workspace each; all of it goes with the table's rows"""
+    run(stub, """
+        import numpy as np, threading
+        a = np.ones((300, 16), np.float32).ctypes.data
+        def search(t, nq, k=5):
+            return L.ndbhip_i8_search(t, a, nq, None, None, 0, k, a, a)
+        empty = stub.stub_in_use()
+        t = table(16, 100_000)
+        rows = stub.stub_in_use()
+        _lib.check(search(t, 4))
+        m, f, kept = stub.stub_mallocs(), stub.stub_frees(), stub.stub_in_use()
+        assert kept > rows
+        for _ in range(5):
+            _lib.check(search(t, 4))
+            _lib.check(search(t, 1))
+        assert (stub.stub_mallocs(), stub.stub_frees(), stub.stub_in_use()) == (m, f, kept)
+        _lib.check(search(t, 200))                      # a larger one: in place of the first
+        assert stub.stub_mallocs() == m + 1 and stub.stub_frees() == f + 1
+        # two at the same time
+        stub.stub_set_sync_ms(300)
+        got = []
+        th = [threading.Thread(target=lambda: got.append(search(t, 4))) for _ in range(2)]
+        [x.start() for x in th]
+        [x.join() for x in th]
+        stub.stub_set_sync_ms(0)
+        assert got == [0, 0] and stub.stub_mallocs() == m + 2
+        _lib.check(search(t, 4)), _lib.check(search(t, 200))
+        assert stub.stub_mallocs() == m + 2
+        # no room: an error, and the next search has its workspace again
+        stub.stub_set_room(stub.stub_in_use())
+        assert search(t, 250, 1000) == _lib.ERR_NOMEM and "room" in _lib.last_error()
+        stub.stub_set_room(1 << 62)
+        _lib.check(search(t, 250, 1000)), _lib.check(search(t, 4))
+        # a workspace of more than a gigabyte is not kept
+        before = stub.stub_in_use()
+        big = table(64, 100_000_000)
+        rows = stub.stub_in_use()
+        _lib.check(L.ndbhip_i8_search(big, a, 256, None, None, 0, 5, a, a))
+        assert stub.stub_in_use() == rows and stub.stub_most() > rows + 3 * 10**9
+        _lib.check(L.ndbhip_i8_destroy(big))
+        assert stub.stub_in_use() == before
+        _lib.check(L.ndbhip_i8_load_device(t, P, 3, 1000, 16, P))
+        _lib.check(L.ndbhip_i8_destroy(t))
+        assert stub.stub_in_use() == empty
+    """)
