@@ -751,7 +751,7 @@ template <int NWQ> struct I8Tile
 };
 
 template <int NWQ, class KIND>
-__global__ __launch_bounds__(128 * NWQ, 2) void
+__global__ __launch_bounds__(128 * NWQ, NWQ == 2 && (KIND::BIAS || KIND::MASK) ? 1 : 2) void
 k_i8_tile(const unsigned char *__restrict__ rows, const unsigned char *__restrict__ queries, uint32_t kp, uint32_t nrt, uint32_t nqt, I8Out o)
 {
 	typedef I8Tile<NWQ> TILE;
