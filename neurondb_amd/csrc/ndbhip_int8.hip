@@ -1444,14 +1444,17 @@ struct I8Adjust
  * A block of threads takes 256 * VEC * U neighbouring columns of one query and reads their scores at once; meanwhile it counts how
  * often the query's list names each of them (the whole list is read per block: it is short next to the columns, and
  * LDS counters need neither a sort nor a hash nor a bound on its length).  Bound by HBM: a score read and written, a bit
- * of mask (64 x 1M fp32: 122 us, 4.3 TB/s).
+ * of mask (64 x 1M fp32: 122 us, 4.3 TB/s).  Without lists (SEEN false) nothing is shared by a block's columns, and a thread takes
+ * one piece: 64 x 333333 and a bias, which the last level cache holds, 38.2 us with four pieces and the counters' LDS, 35.0 with two,
+ * 31.6 with one (torch's addition 32.6), 64 x 1M 107.7, 106.9, 105.4, in 16 bits 80, 76, 71; it loses where blocks have little to do
+ * (2048 x 3001 and mask and bias: 8.7 -> 9.3).
  */
-template <class T, int U>
+template <class T, int U, bool SEEN>
 __global__ __launch_bounds__(256) void
 k_scores_adjust(const I8Adjust a)
 {
 	constexpr int VEC = 16 / sizeof(T), COLS = 256 * VEC * U;
-	__shared__ __attribute__((aligned(16))) uint32_t cnt[COLS];
+	__shared__ __attribute__((aligned(16))) uint32_t cnt[SEEN ? COLS : 4];
 	const int64_t q = a.q0 + (int64_t) blockIdx.y;
 	const int64_t c0 = (int64_t) blockIdx.x * COLS;
 	const int	m = (int) min((int64_t) COLS, a.n - c0);
@@ -1496,7 +1499,7 @@ k_scores_adjust(const I8Adjust a)
 					add[u][i] = e + i < m ? bv[e + i] : 0.0f;
 		}
 	}
-	const int64_t lo = a.seen_off ? max(a.seen_off[q], (int64_t) 0) : 0, hi = a.seen_off ? min(a.seen_off[q + 1], a.nseen) : 0;
+	const int64_t lo = SEEN ? max(a.seen_off[q], (int64_t) 0) : 0, hi = SEEN ? min(a.seen_off[q + 1], a.nseen) : 0;
 	const bool	seen = hi > lo;
 	float		repeat = 1.0f, presence = 0.0f, frequency = 0.0f;
 
@@ -2441,9 +2444,10 @@ template <class T>
 static void
 scores_adjust_launch(I8Adjust a)
 {
-	/* columns a block takes: many scores 4096 (fp32) or 8192 (16 bits), which halves the list's reads; else half of that */
+	/* columns a block takes: many scores 4096 (fp32) or 8192 (16 bits), which halves the list's reads; else half of that; without
+	 * lists 1024 (2048) */
 	constexpr int VEC = 16 / sizeof(T);
-	const int	u = (int64_t) a.nq * a.n >= ((int64_t) 4 << 20) ? 4 : 2, cols = 256 * VEC * u;
+	const int	u = !a.seen_off ? 1 : (int64_t) a.nq * a.n >= ((int64_t) 4 << 20) ? 4 : 2, cols = 256 * VEC * u;
 
 	/* (64 bits: behind 2^31 - 65536 queries the next start is not an int) */
 	for (int64_t q0 = 0; q0 < a.nq; q0 += 65535)
@@ -2452,9 +2456,11 @@ scores_adjust_launch(I8Adjust a)
 
 		a.q0 = (int) q0;
 		if (u == 4)
-			hipLaunchKernelGGL((k_scores_adjust<T, 4>), grid, dim3(256), 0, g.stream, a);
+			hipLaunchKernelGGL((k_scores_adjust<T, 4, true>), grid, dim3(256), 0, g.stream, a);
+		else if (u == 2)
+			hipLaunchKernelGGL((k_scores_adjust<T, 2, true>), grid, dim3(256), 0, g.stream, a);
 		else
-			hipLaunchKernelGGL((k_scores_adjust<T, 2>), grid, dim3(256), 0, g.stream, a);
+			hipLaunchKernelGGL((k_scores_adjust<T, 1, false>), grid, dim3(256), 0, g.stream, a);
 	}
 }
 

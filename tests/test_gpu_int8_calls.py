@@ -1,4 +1,5 @@
 """The way from Python and C to the 8-bit kernels, on the device: what a call costs and leaves behind."""
+import math
 import threading
 import time
 
@@ -33,6 +34,38 @@ def test_one_term_on_few_scores_costs_no_more_than_an_addition(nq, n):
     s, b = torch.randn(nq, n, device="cuda"), torch.randn(n, device="cuda")
     own, plain = us([lambda: nd.adjust_scores(s, bias=b), lambda: s + b[None]])
     assert own < 1.33 * plain, (own, plain)
+
+
+def test_one_term_on_scores_that_a_cache_holds_costs_no_more_than_an_addition():
+    """(the kernel with the lists' counters took 1.17 times the addition)"""
+    s, b = torch.randn(64, 333_333, device="cuda"), torch.randn(333_333, device="cuda")
+    own, plain = us([lambda: nd.adjust_scores(s, bias=b), lambda: s + b[None]], reps=100)
+    assert own < 1.1 * plain, (own, plain)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 3, 7, 1023, 1024, 1025, 2047, 2048, 2049, 4100])
+def test_terms_without_lists(n, dtype):
+    """one rounding to fp32 for the bias and one to the type, so equal bit for bit; what lies beside the result stays"""
+    nq = 5
+    g = torch.Generator().manual_seed(n)
+    s = torch.randn(nq, n, generator=g).to(dtype)
+    s[0, 0], s[1, n - 1], s[2, n // 2] = float("nan"), float("-inf"), float("inf")
+    b, bq = torch.randn(n, generator=g), torch.randn(nq, n, generator=g)
+    bits = torch.rand(nq, (n + 31) // 32 * 32, generator=g) < 0.5
+    bits[3] = False
+    words = (bits.view(nq, -1, 32).long() << torch.arange(32)).sum(2)
+    words = torch.where(words >= 2 ** 31, words - 2 ** 32, words).int()
+    bits = bits[:, :n]
+    for bias in (None, b, bq):
+        for mask in (None, words, words[:1]):
+            want = s.float() if bias is None else s.float() + bias
+            if mask is not None:
+                want = want.masked_fill(~bits if mask.shape[0] > 1 else ~bits[:1], float("-inf"))
+            out = torch.full((nq + 1, n + 9), 7.0, dtype=dtype, device="cuda")
+            nd.adjust_scores(s.cuda(), bias=None if bias is None else bias.cuda(), mask=None if mask is None else mask.cuda(), out=out[:nq, 3:3 + n])
+            assert torch.equal(out[:nq, 3:3 + n].cpu().nan_to_num(9.0, math.inf, -math.inf), want.to(dtype).nan_to_num(9.0, math.inf, -math.inf))
+            assert bool((out[nq] == 7).all()) and bool((out[:, :3] == 7).all()) and bool((out[:, 3 + n:] == 7).all())
 
 
 def test_a_saved_tensor_is_not_changed_unseen():
