@@ -50,7 +50,7 @@ class _Torch:
         import torch
         if not _lib._inited:
             ensure_init(torch.cuda.current_device())
-        self.torch = torch
+        self.torch, self.Tensor = torch, torch.Tensor
         self.types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
         self.floats = (torch.float32, torch.float16, torch.bfloat16)
         self.f32, self.i8, self.i32, self.i64 = (torch.float32,), (torch.int8,), (torch.int32,), (torch.int64,)
@@ -102,7 +102,7 @@ def _call(fn, *args):
 def _tensor(t, name, dtypes, ndim, followed=False):
     """checks what every tensor argument has to be; followed: it may be one whose gradients autograd is to find"""
     T = _state
-    if not isinstance(t, T.torch.Tensor):
+    if not isinstance(t, T.Tensor):
         raise _bad(f"{name} must be a torch tensor")
     if t.device != T.device:
         raise _bad(f"{name} is on {t.device}, the library on {T.device}")
@@ -115,7 +115,7 @@ def _tensor(t, name, dtypes, ndim, followed=False):
     return t
 
 
-def _written(*out):
+def _written(out):
     """the caller's own tensors that a call has written into: what autograd has saved of them is another version now"""
     for t in out:
         if not t.is_inference():
@@ -152,7 +152,9 @@ def quantize_rows(x, codes=None, scales=None):
     T = _torch()
     x, stride = _rows(_tensor(x, "x", T.floats, 2))
     n, dim = x.shape
-    given = [t for t in (codes, scales) if t is not None]
+    given = None
+    if codes is not None or scales is not None:
+        given = [t for t in (codes, scales) if t is not None]
     if codes is None:
         codes = T.torch.empty((n, dim), dtype=T.torch.int8, device=T.device)
         cstride = dim
@@ -165,7 +167,8 @@ def quantize_rows(x, codes=None, scales=None):
     if codes.shape != x.shape or scales.shape[0] != n or not scales.is_contiguous():
         raise _bad("codes must be [n, dim] and scales [n], contiguous")
     _call(T.lib.ndbhip_i8_quantize_device, _p(x), T.types[x.dtype], n, dim, stride, _p(codes), cstride, _p(scales))
-    _written(*given)
+    if given is not None:
+        _written(given)
     return codes, scales
 
 
@@ -177,14 +180,15 @@ def dequantize_rows(codes, scales, dtype=None, out=None):
     n, dim = codes.shape
     if scales.shape[0] != n:
         raise _bad("a scale for every row")
-    given = () if out is None else (out,)
+    given = out
     if out is None:
         out = T.torch.empty((n, dim), dtype=dtype or T.torch.float32, device=T.device)
     _tensor(out, "out", T.floats, 2)
     if out.shape != codes.shape or dtype not in (None, out.dtype):
         raise _bad("out must have the codes' shape and the dtype asked for")
     _call(T.lib.ndbhip_i8_dequantize_device, _p(codes), stride, _p(scales), n, dim, _p(out), T.types[out.dtype], _out_rows(out, "out"))
-    _written(*given)
+    if given is not None:
+        _written((given,))
     return out
 
 
@@ -310,7 +314,8 @@ class Int8Table:
             raise _bad(f"queries must be [nq, {self.dim}]")
         if (q.dtype == T.torch.int8) != (scales is not None) or scales is not None and scales.shape[0] != q.shape[0]:
             raise _bad("int8 queries come as (codes [nq, dim], scales [nq]), others alone")
-        _int(q.shape[0], "the number of queries")
+        if q.shape[0] >= 1 << 31:
+            _int(q.shape[0], "the number of queries")
         return T, q, stride, scales
 
     def _workspace(self, T, nq, k):
@@ -329,7 +334,7 @@ class Int8Table:
         T, q, stride, qs = self._queries(queries)
         nq, n = q.shape[0], self._n
         bias = _bias_arg(bias, n)
-        given = () if out is None else (out,)
+        given = out
         if out is None:
             out = T.torch.empty((nq, n), dtype=dtype or T.torch.float32, device=T.device)
         _tensor(out, "out", T.floats, 2)
@@ -339,7 +344,8 @@ class Int8Table:
         ws, wsb = self._workspace(T, nq, 0)
         _call(T.lib.ndbhip_i8_product_device, self._h, _p(q), T.types[q.dtype], _p(qs), nq, stride, _p(bias), _p(out), T.types[out.dtype],
               ostride, _p(ws), wsb)
-        _written(*given)
+        if given is not None:
+            _written((given,))
         return out
 
     def search(self, queries, k, bias=None, mask=None):
@@ -349,7 +355,9 @@ class Int8Table:
         if isinstance(queries, np.ndarray):
             return self._search_host(queries, _int(k, "k"), bias, mask)
         T, q, stride, qs = self._queries(queries)
-        nq, n, k = q.shape[0], self._n, _int(k, "k")
+        nq, n, k = q.shape[0], self._n, int(k)
+        if not 0 < k < 1 << 31:
+            raise _bad(f"k is {k}")
         bias = _bias_arg(bias, n)
         mask, mstride = _mask_arg(mask, nq, n)
         ws, wsb = self._workspace(T, nq, k)
