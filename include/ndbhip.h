@@ -758,7 +758,8 @@ int			ndbhip_quant_fp16(const float *in, uint16_t *out, int64_t n);
  * (ndbhip_i8_workspace; 256-byte aligned; its contents mean nothing before or after, and it must live until the call's kernels
  * have run — for a captured graph, as long as the graph is replayed).  ndbhip_i8_load* and _destroy wait for nothing but
  * their own work: call them while no other call on the table is in flight and no graph that reads it will be replayed.
- * The calling thread's current HIP device is the same after a call as before it.
+ * The calling thread's current HIP device is the same after a call as before it.  What a process calls first must not be under
+ * capture: it sets the library up.
  * Any dimension 1 .. 32767, any number of rows below 2^31 - 256, any strides and alignments of an element's own size. */
 /* ------------------------------------------------------------------ */
 typedef struct ndbhip_i8 ndbhip_i8;		/* device-resident table of 8-bit rows */
@@ -804,12 +805,14 @@ int			ndbhip_i8_search(const ndbhip_i8 *t, const float *queries, int nq, const f
 							 int k, int64_t *ids, float *scores);
 
 /* Penalties, biases and masks over a matrix of scores [nq][n] (fp32, fp16 or bf16; arithmetic in fp32, rounded once), to
- * another matrix of the type or in place (d_out == d_scores with the same stride; no other overlap):
+ * another matrix of the type or in place (d_out == d_scores with the same stride):
  *   seen       query q has been given ids d_seen_ids[d_seen_off[q] .. d_seen_off[q + 1]) before, in any order, an id once for
  *              every time; what lies outside the n_seen ids there are is not read, ids outside 0 .. n - 1 count for nothing.  d_penalties[q] = {repeat, presence, frequency}, repeat > 0.  For an id
  *              given c > 0 times: s = s > 0 ? s / repeat : s * repeat, then s = s - (presence + c * frequency).  d_seen_off NULL: none
  *   bias       s = s + bias; bias_stride from one query's to the next, 0 = one for all; NULL: none
- *   mask       bit 0: s = -infinity, whatever it was; as above; NULL: none */
+ *   mask       bit 0: s = -infinity, whatever it was; as above; NULL: none
+ * Higher is better, as for all scores here: distances (ndbhip_batch_distance for L2 and cosine) have to be negated first, or
+ * what is masked would rank first.  d_out otherwise shares no element with d_scores; rows of the two may lie between each other. */
 int			ndbhip_scores_adjust_device(const void *d_scores, int dtype, int nq, int64_t n, int64_t stride, const int64_t *d_seen_off,
 										const int32_t *d_seen_ids, int64_t n_seen, const float *d_penalties, const float *d_bias, int64_t bias_stride,
 										const uint32_t *d_mask, int64_t mask_stride, void *d_out, int64_t out_stride);

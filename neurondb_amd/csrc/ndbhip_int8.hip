@@ -724,17 +724,21 @@ i8_lds(const void *p)
  * in registers.  Both operands pass through LDS in stages of 64 dimensions (2 KiB a block of 32 rows
  * or queries, copied as they lie in memory; an LDS read is 16 bytes a lane without conflicts), a ring of NBUF.
  *
- * Two waves a SIMD do not hide each other's waits (they meet at the same barriers), so the stream is pipelined by hand.  A
- * stage is two halves of 32 dimensions
- * (one matrix instruction deep): while one half is multiplied, the operands of the next are read, also across the
- * barrier that opens the next stage.  Tiles follow each other without a gap: the ring runs into the next tile of the
- * block, whose first operands are in registers when the sums of this one are written out.
+ * Two waves a SIMD do not hide each other's waits (those of a wide tile meet at the same barriers), so the stream is pipelined
+ * by hand.  A stage is two halves of 32 dimensions (one matrix instruction deep): while one half is multiplied, the operands of
+ * the next are read, also across the barrier that opens the next stage.  The ring runs into the next tile of the block, whose
+ * first operands are in registers when the sums of this one are written out.
  *
  * Row scales, query scales, biases and mask words of a tile come through LDS the same way, with the copies of its first stage: a load
  * of the wave's own would have to wait for every copy requested before it (requests retire in order).
  *
- * Bound by the matrix pipe and the clock it runs at: 1024 x 1M x 768 to maxima 724 us (2.2 POP/s, the pipe busy 55 % of the
- * cycles; 690 on another box, and 570 there on zeros), 1024 x 131072 x 1536 to fp32 scores 214, 77 x 50021 x 300 bf16 11.
+ * Scores are the gap that is left: they count among the requests that the next stage waits for, and retire in order, so a
+ * tile's 128 stores a wave (64 in 16 bits) are nearly all done before the next tile's first half stage ends.
+ *
+ * Bound by LDS and the matrix pipe together, and the clock they run at: a half stage moves 48 KiB out of LDS and 16 in, 512
+ * cycles at 128 bytes each, and is 512 cycles of the pipe.  1024 x 1M x 768 to maxima 724 us (2.2 POP/s, the pipe busy 55 % of
+ * the cycles; 690 on another box, and 570 there on zeros; 635 without the epilogue, 449 without the operands' LDS reads as well),
+ * 1024 x 131072 x 1536 to fp32 scores 217, 77 x 50021 x 300 bf16 11.
  */
 #define I8_TR 8					/* blocks of rows in a tile */
 #define I8_NBUF 3
